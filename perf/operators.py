@@ -140,30 +140,38 @@ _NODES = {  # operator -> graph node, its inputs in order
 _NUMPY = {torch.float16: "float16", torch.float32: "float32", torch.int8: "int8"}
 
 
-def _compile(state):
-    """The one-node graph of a case, compiled, with the state's tensors bound
-    to its inputs and buffers of its own bound to its outputs."""
+@functools.cache
+def _engine(op, names, shapes, dtypes, outputs, attributes):
+    """The compiled one-node graph of a case; a program compiles its graph
+    once and binds each request's tensors to a context."""
     import cutriton_b200 as ct
 
+    model = ct.Model()
+    for name, shape, dtype in zip(names, shapes, dtypes):
+        model.add_input(name, list(shape), dtype=dtype, layout="")
+    model.add_node("node", op, list(names), list(outputs), **dict(attributes))
+    for name in outputs:
+        model.add_output(name)
+    return ct.build_engine(model, enable_profiling=False, tuning_mode=ct.TUNING_DISABLED)
+
+
+def _compile(state):
+    """A context of the case's graph with the state's tensors bound to its
+    inputs and buffers of its own bound to its outputs."""
     case, tensors = state["case"], state["tensors"]
     op_type, names = _NODES[case["op"]]
-    names = [name for name in names if name in tensors]
-    model = ct.Model()
-    for name in names:
-        model.add_input(name, list(tensors[name].shape), dtype=_NUMPY[tensors[name].dtype], layout="")
+    names = tuple(name for name in names if name in tensors)
+    attributes = {}
     if case["op"] == "quantize":
         outputs = {"q": torch.empty(case["m"], case["k"], dtype=torch.int8, device="cuda"),
                    "q_scale": torch.empty(case["m"], dtype=torch.float32, device="cuda")}
-        model.add_node("node", op_type, names, list(outputs))
     else:
         outputs = {"y": torch.empty(case["m"], case["n"], dtype=torch.float16, device="cuda")}
-        attributes = {"transB": 1}
+        attributes["transB"] = 1
         if "act" in case:
             attributes["activation"] = case["act"]
-        model.add_node("node", op_type, names, list(outputs), **attributes)
-    for name in outputs:
-        model.add_output(name)
-    engine = ct.build_engine(model, enable_profiling=False, tuning_mode=ct.TUNING_DISABLED)
+    engine = _engine(op_type, names, tuple(tuple(tensors[name].shape) for name in names),
+                     tuple(_NUMPY[tensors[name].dtype] for name in names), tuple(outputs), tuple(attributes.items()))
     context = engine.create_context()
     for name in names:
         context.bind_tensor(name, tensors[name])
