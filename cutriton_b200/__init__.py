@@ -26,11 +26,11 @@ PACK_DIR = PACKAGE_DIR / "pack"
 OK, INVALID_ARGUMENT, NOT_FOUND, ALREADY_EXISTS, UNSUPPORTED, SHAPE_ERROR, RUNTIME_ERROR, INTERNAL = range(8)
 ERROR_NAMES = ["OK", "InvalidArgument", "NotFound", "AlreadyExists", "Unsupported", "ShapeError",
                "RuntimeError", "Internal"]
-FLOAT32, FLOAT16, INT32, INT64 = 1, 2, 3, 4
+FLOAT32, FLOAT16, INT32, INT64, INT8 = 1, 2, 3, 4, 5
 TUNING_DISABLED, TUNING_USE_CACHE, TUNING_TUNE_ON_MISS, TUNING_FORCE_RETUNE = range(4)
 MAX_RANK = 8
 
-_NUMPY_DTYPES = {FLOAT32: np.float32, FLOAT16: np.float16, INT32: np.int32, INT64: np.int64}
+_NUMPY_DTYPES = {FLOAT32: np.float32, FLOAT16: np.float16, INT32: np.int32, INT64: np.int64, INT8: np.int8}
 _DTYPE_OF_NUMPY = {np.dtype(v): k for k, v in _NUMPY_DTYPES.items()}
 
 

@@ -65,15 +65,22 @@ Status TargetCapability(int device_id, int* capability) {
   return status;
 }
 
-// Why the value `name` cannot take part in a cuda_sm100 launch, or "".
-std::string TensorProblem(const Graph& graph, const std::string& name, const Device& device) {
+// Ops whose shape inference checks 8-bit operands (and the view, which moves
+// no bytes); every other op takes float tensors only.
+bool TakesInt8(const std::string& op) {
+  return op == "QuantizeRows" || op == "QGemm" || op == "QGatedGemm" || op == "Flatten";
+}
+
+// Why the value `name` cannot take part in a cuda_sm100 launch of `op`, or "".
+std::string TensorProblem(const Graph& graph, const std::string& op, const std::string& name, const Device& device) {
   const ValueDesc* value = graph.FindValue(name);
   if (value == nullptr) return "'" + name + "' has no description";
   const Status valid = value->tensor.Validate();
   if (!valid.ok()) return "'" + name + "': " + valid.message();
   const DataType dtype = value->tensor.dtype;
-  if (dtype != DataType::kFloat32 && dtype != DataType::kFloat16) {
-    return "'" + name + "' is " + DataTypeName(dtype) + " (kernels take float32 / float16)";
+  if (dtype != DataType::kFloat32 && dtype != DataType::kFloat16 && !(dtype == DataType::kInt8 && TakesInt8(op))) {
+    return "'" + name + "' is " + DataTypeName(dtype) + " (kernels take float32 / float16" +
+           (TakesInt8(op) ? " / int8)" : ")");
   }
   if (value->tensor.device_type != device.type || value->tensor.device_id != device.id) {
     return "'" + name + "' is placed on another device";
@@ -170,7 +177,7 @@ Status CheckCudaNode(const Node& node, const Graph& graph, const BackendOptions&
   }
   for (const auto* names : {&node.inputs(), &node.outputs()}) {
     for (const std::string& name : *names) {
-      const std::string problem = TensorProblem(graph, name, options.device);
+      const std::string problem = TensorProblem(graph, node.op_type(), name, options.device);
       if (!problem.empty()) return Status::Unsupported(who + problem);
     }
   }
@@ -355,6 +362,14 @@ class CudaSm100Backend final : public Backend {
       const std::string projected = temp("gemm", 0);
       steps.push_back({"Gemm", in, {projected}});
       steps.push_back({"Gelu", {projected}, {out}});
+    } else if (op == "GatedGemm") {
+      const std::string gate = temp("gate", 0);
+      const std::string up = temp("up", 1);
+      const std::string activated = temp("activated", 2);
+      steps.push_back({"Gemm", {in[0], in[1]}, {gate}});
+      steps.push_back({"Gemm", {in[0], in[2]}, {up}});
+      steps.push_back({GetIntAttribute(node, "activation", 0) == 0 ? "Silu" : "Gelu", {gate}, {activated}});
+      steps.push_back({"Mul", {activated, up}, {out}});
     } else if (op == "SkipLayerNormalization") {
       const std::string sum = temp("add", 0);
       steps.push_back({"Add", {in[0], in[1]}, {sum}});

@@ -161,7 +161,8 @@ Status EncodeTensorMap(const Tensor& tensor, const KernelArgumentSource& s, CUte
   switch (desc.dtype) {
     case DataType::kFloat32: type = CU_TENSOR_MAP_DATA_TYPE_FLOAT32; break;
     case DataType::kFloat16: type = CU_TENSOR_MAP_DATA_TYPE_FLOAT16; break;
-    default: return Status::Unsupported("tensor_map supports float32/float16 tensors");
+    case DataType::kInt8: type = CU_TENSOR_MAP_DATA_TYPE_UINT8; break;
+    default: return Status::Unsupported("tensor_map supports float32 / float16 / int8 tensors");
   }
   const std::size_t element = ElementSize(desc.dtype);
   cuuint64_t dims[5];
@@ -238,6 +239,8 @@ Status BindArguments(const KernelInvocation& inv, KernelContext* context, BoundP
     const Tensor* tensor = nullptr;
     switch (s.kind) {
       case KernelArgumentSourceKind::kInput:
+        // An optional input that the node does not have is a null pointer.
+        if (s.optional && s.index >= 0 && static_cast<std::size_t>(s.index) >= inv.inputs.size()) break;
         CUTRITON_RETURN_IF_ERROR(TensorAt(inv.inputs, s.index, s.prepack, context, &tensor));
         slot.pointer = DeviceAddress(*tensor);
         break;

@@ -188,6 +188,7 @@ KernelArgumentSpec ParseArgument(const json::Value& v) {
   s.default_int = IntOr(src, "default", 0);
   s.default_float = DoubleOr(src, "default", 0.0);
   if (const auto* prepack = src.find("prepack")) s.prepack = prepack->str();
+  if (s.kind == KernelArgumentSourceKind::kInput) s.optional = IntOr(src, "optional", 0) != 0;
   if (s.kind == KernelArgumentSourceKind::kTensorMap) {
     const std::string& tensor = src.at("tensor").str();
     if (tensor != "input" && tensor != "output") {

@@ -52,6 +52,7 @@ DataType ToDataType(int dtype) {
     case CTB_DTYPE_FLOAT16: return DataType::kFloat16;
     case CTB_DTYPE_INT32: return DataType::kInt32;
     case CTB_DTYPE_INT64: return DataType::kInt64;
+    case CTB_DTYPE_INT8: return DataType::kInt8;
     default: return DataType::kUnknown;
   }
 }
@@ -62,6 +63,7 @@ int FromDataType(DataType dtype) {
     case DataType::kFloat16: return CTB_DTYPE_FLOAT16;
     case DataType::kInt32: return CTB_DTYPE_INT32;
     case DataType::kInt64: return CTB_DTYPE_INT64;
+    case DataType::kInt8: return CTB_DTYPE_INT8;
     default: return CTB_DTYPE_UNKNOWN;
   }
 }

@@ -10,6 +10,7 @@ const char* DataTypeName(DataType dtype) {
     case DataType::kFloat16: return "float16";
     case DataType::kInt32: return "int32";
     case DataType::kInt64: return "int64";
+    case DataType::kInt8: return "int8";
     case DataType::kUnknown: break;
   }
   return "unknown";
@@ -25,6 +26,7 @@ std::size_t ElementSize(DataType dtype) {
     case DataType::kInt32: return 4;
     case DataType::kFloat16: return 2;
     case DataType::kInt64: return 8;
+    case DataType::kInt8: return 1;
     case DataType::kUnknown: break;
   }
   return 0;

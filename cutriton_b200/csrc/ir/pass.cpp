@@ -156,6 +156,121 @@ Status InferGemm(Graph* graph, const Node& node) {
   return graph->SetValueDesc(node.outputs()[0], std::move(out));
 }
 
+// ---- gated and 8-bit products ----------------------------------------------------
+
+// The weight `name` of a product over x's K columns: [K, N], or [N, K] with
+// transB. Gives N.
+Status CheckWeight(const Graph& graph, const Node& node, const std::string& name, int64_t k, DataType dtype,
+                   int64_t* n) {
+  const ValueDesc* w = graph.FindValue(name);
+  const std::string who = node.op_type() + " weight '" + name + "' ";
+  if (w == nullptr || w->tensor.shape.size() != 2) return Status::ShapeError(who + "must be a rank-2 tensor");
+  if (w->tensor.dtype != dtype) return Status::ShapeError(who + "must be " + DataTypeName(dtype));
+  const bool tb = GetIntAttribute(node, "transB", 0) != 0;
+  const auto& s = w->tensor.shape;
+  if ((tb ? s[1] : s[0]) != k) return Status::ShapeError(who + "does not match the inner dimension");
+  *n = tb ? s[0] : s[1];
+  return Status::OK();
+}
+
+Status CheckVector(const Graph& graph, const Node& node, const std::string& name, int64_t length, DataType dtype) {
+  const ValueDesc* v = graph.FindValue(name);
+  if (v == nullptr || v->tensor.shape != std::vector<int64_t>{length} || v->tensor.dtype != dtype) {
+    return Status::ShapeError(node.op_type() + " '" + name + "' must be " + DataTypeName(dtype) + " [" +
+                              std::to_string(length) + "]");
+  }
+  return Status::OK();
+}
+
+// activation: 0 = SiLU, 1 = erf-GELU. transB: 0 or 1; transA does not exist.
+Status CheckProductAttributes(const Node& node, bool gated) {
+  const int64_t tb = GetIntAttribute(node, "transB", 0);
+  if ((tb != 0 && tb != 1) || GetIntAttribute(node, "transA", 0) != 0) {
+    return Status::Unsupported(node.op_type() + ": transB must be 0 or 1, transA 0");
+  }
+  const int64_t activation = GetIntAttribute(node, "activation", 0);
+  if (gated && activation != 0 && activation != 1) {
+    return Status::Unsupported(node.op_type() + ": activation must be 0 (SiLU) or 1 (erf-GELU)");
+  }
+  return Status::OK();
+}
+
+// x [M, K], w_gate, w_up -> act(x . w_gate) * (x . w_up), [M, N].
+Status InferGatedGemm(Graph* graph, const Node& node) {
+  CUTRITON_RETURN_IF_ERROR(CheckProductAttributes(node, true));
+  const ValueDesc* x = graph->FindValue(node.inputs()[0]);
+  if (x == nullptr || x->tensor.shape.size() != 2) return Status::ShapeError("GatedGemm expects a rank-2 input");
+  const int64_t k = x->tensor.shape[1];
+  int64_t n = 0, n_up = 0;
+  CUTRITON_RETURN_IF_ERROR(CheckWeight(*graph, node, node.inputs()[1], k, x->tensor.dtype, &n));
+  CUTRITON_RETURN_IF_ERROR(CheckWeight(*graph, node, node.inputs()[2], k, x->tensor.dtype, &n_up));
+  if (n != n_up) return Status::ShapeError("GatedGemm gate and up weights must have the same width");
+  TensorDesc out = Derived(x->tensor, {x->tensor.shape[0], n}, "");
+  CUTRITON_RETURN_IF_ERROR(out.Validate());
+  return graph->SetValueDesc(node.outputs()[0], std::move(out));
+}
+
+// x [M, K] float16 -> q [M, K] int8, scale [M] float32.
+Status InferQuantizeRows(Graph* graph, const Node& node) {
+  const ValueDesc* x = graph->FindValue(node.inputs()[0]);
+  if (x == nullptr || x->tensor.shape.size() != 2 || x->tensor.dtype != DataType::kFloat16) {
+    return Status::ShapeError("QuantizeRows expects a rank-2 float16 input");
+  }
+  TensorDesc q = Derived(x->tensor, x->tensor.shape, "");
+  q.dtype = DataType::kInt8;
+  TensorDesc scale = Derived(x->tensor, {x->tensor.shape[0]}, "");
+  scale.dtype = DataType::kFloat32;
+  CUTRITON_RETURN_IF_ERROR(q.Validate());
+  CUTRITON_RETURN_IF_ERROR(graph->SetValueDesc(node.outputs()[0], std::move(q)));
+  return graph->SetValueDesc(node.outputs()[1], std::move(scale));
+}
+
+// The 8-bit left operand and its row scales (inputs 0 and 1). K is limited so
+// that a sum of K products of any two 8-bit values fits 32 bits.
+Status CheckQuantizedRows(const Graph& graph, const Node& node, int64_t* m, int64_t* k) {
+  const ValueDesc* x = graph.FindValue(node.inputs()[0]);
+  if (x == nullptr || x->tensor.shape.size() != 2 || x->tensor.dtype != DataType::kInt8) {
+    return Status::ShapeError(node.op_type() + " expects a rank-2 int8 input");
+  }
+  *m = x->tensor.shape[0];
+  *k = x->tensor.shape[1];
+  if (*k >= 131072) return Status::Unsupported(node.op_type() + ": the inner dimension must be below 131072");
+  return CheckVector(graph, node, node.inputs()[1], *m, DataType::kFloat32);
+}
+
+Status SetProduct(Graph* graph, const Node& node, int64_t m, int64_t n) {
+  TensorDesc out = Derived(graph->FindValue(node.inputs()[0])->tensor, {m, n}, "");
+  out.dtype = DataType::kFloat16;
+  CUTRITON_RETURN_IF_ERROR(out.Validate());
+  return graph->SetValueDesc(node.outputs()[0], std::move(out));
+}
+
+// q [M, K], scale [M], w, w_scale [N] (, bias [N]) -> [M, N] float16.
+Status InferQGemm(Graph* graph, const Node& node) {
+  CUTRITON_RETURN_IF_ERROR(CheckProductAttributes(node, false));
+  int64_t m = 0, k = 0, n = 0;
+  CUTRITON_RETURN_IF_ERROR(CheckQuantizedRows(*graph, node, &m, &k));
+  CUTRITON_RETURN_IF_ERROR(CheckWeight(*graph, node, node.inputs()[2], k, DataType::kInt8, &n));
+  CUTRITON_RETURN_IF_ERROR(CheckVector(*graph, node, node.inputs()[3], n, DataType::kFloat32));
+  if (node.inputs().size() == 5) {
+    CUTRITON_RETURN_IF_ERROR(CheckVector(*graph, node, node.inputs()[4], n, DataType::kFloat16));
+  }
+  return SetProduct(graph, node, m, n);
+}
+
+// q [M, K], scale [M], w_gate, gate_scale [N], w_up, up_scale [N] -> [M, N] float16.
+Status InferQGatedGemm(Graph* graph, const Node& node) {
+  CUTRITON_RETURN_IF_ERROR(CheckProductAttributes(node, true));
+  int64_t m = 0, k = 0, n = 0, n_up = 0;
+  CUTRITON_RETURN_IF_ERROR(CheckQuantizedRows(*graph, node, &m, &k));
+  CUTRITON_RETURN_IF_ERROR(CheckWeight(*graph, node, node.inputs()[2], k, DataType::kInt8, &n));
+  CUTRITON_RETURN_IF_ERROR(CheckVector(*graph, node, node.inputs()[3], n, DataType::kFloat32));
+  CUTRITON_RETURN_IF_ERROR(CheckWeight(*graph, node, node.inputs()[4], k, DataType::kInt8, &n_up));
+  CUTRITON_RETURN_IF_ERROR(CheckVector(*graph, node, node.inputs()[5], n_up, DataType::kFloat32));
+  if (n != n_up) return Status::ShapeError("QGatedGemm gate and up weights must have the same width");
+  return SetProduct(graph, node, m, n);
+}
+
 Status CheckNormParams(const Graph& graph, const std::string& x_name,
                        const std::string& scale_name, const std::string* bias_name,
                        int64_t axis) {
@@ -384,6 +499,49 @@ class ConvResidualFusionPass final : public GraphPass {
   }
 };
 
+// Gemm -> Silu | Gelu, times a second Gemm of the same input => GatedGemm.
+class GatedGemmFusionPass final : public GraphPass {
+ public:
+  const char* name() const override { return "gated_gemm_fusion"; }
+  Status Run(Graph* graph) const override {
+    return RewriteToFixpoint(graph, [](Graph* g, const auto& consumers, Node& mul, std::vector<int>* removed) {
+      if (mul.op_type() != "Mul" || mul.inputs().size() != 2 || mul.outputs().size() != 1) return false;
+      // The node that makes `value` for this op alone.
+      const auto producer = [&](const std::string& value) -> const Node* {
+        if (IsGraphOutput(*g, value) || SoleConsumer(consumers, value) < 0) return nullptr;
+        for (const Node& n : g->nodes()) {
+          if (n.outputs().size() == 1 && n.outputs()[0] == value) return &n;
+        }
+        return nullptr;
+      };
+      const auto half_gemm = [&](const Node* n) {
+        if (n == nullptr || (n->op_type() != "Gemm" && n->op_type() != "MatMul") || n->inputs().size() != 2) return false;
+        const ValueDesc* v = g->FindValue(n->outputs()[0]);
+        return v != nullptr && v->tensor.dtype == DataType::kFloat16 && GetIntAttribute(*n, "transA", 0) == 0;
+      };
+      for (int side = 0; side < 2; ++side) {
+        const Node* act = producer(mul.inputs()[side]);
+        const Node* up = producer(mul.inputs()[1 - side]);
+        if (act == nullptr || (act->op_type() != "Silu" && act->op_type() != "Gelu") || act->inputs().size() != 1) continue;
+        const Node* gate = producer(act->inputs()[0]);
+        if (!half_gemm(gate) || !half_gemm(up) || gate == up || gate->inputs()[0] != up->inputs()[0]) continue;
+        const int64_t tb = GetIntAttribute(*gate, "transB", 0);
+        if (tb != GetIntAttribute(*up, "transB", 0)) continue;
+        const int64_t activation = act->op_type() == "Silu" ? 0 : 1;
+        std::vector<std::string> inputs = {gate->inputs()[0], gate->inputs()[1], up->inputs()[1]};
+        *removed = {gate->id(), act->id(), up->id()};
+        mul.set_name(gate->name() + "_gated");
+        mul.set_op_type("GatedGemm");
+        mul.set_inputs(std::move(inputs));
+        mul.SetAttribute("activation", activation);
+        mul.SetAttribute("transB", tb);
+        return true;
+      }
+      return false;
+    });
+  }
+};
+
 class GemmGeluFusionPass final : public GraphPass {
  public:
   const char* name() const override { return "gemm_gelu_fusion"; }
@@ -482,8 +640,8 @@ class StaticShapeValidationPass final : public GraphPass {
 
 Status RegisterBuiltinOpSchemas() {
   auto& registry = OpSchemaRegistry::Global();
-  auto add = [&](const char* op, std::size_t lo, std::size_t hi, ShapeInferenceFunction fn) {
-    const Status status = registry.Register(OpSchema{op, lo, hi, 1, std::move(fn)});
+  auto add = [&](const char* op, std::size_t lo, std::size_t hi, ShapeInferenceFunction fn, std::size_t outputs = 1) {
+    const Status status = registry.Register(OpSchema{op, lo, hi, outputs, std::move(fn)});
     return status.code() == ErrorCode::kAlreadyExists ? Status::OK() : status;
   };
   CUTRITON_RETURN_IF_ERROR(add("Conv", 2, 2, InferConv));
@@ -491,16 +649,21 @@ Status RegisterBuiltinOpSchemas() {
   CUTRITON_RETURN_IF_ERROR(add("FusedConvBatchNormRelu", 6, 6, InferConv));
   CUTRITON_RETURN_IF_ERROR(add("FusedConvBatchNormAddRelu", 7, 7, InferConvAddRelu));
   CUTRITON_RETURN_IF_ERROR(add("BatchNormalization", 5, 5, InferLikeFirstInput));
-  for (const char* op : {"Relu", "Gelu", "Softmax"}) {
+  for (const char* op : {"Relu", "Gelu", "Silu", "Softmax"}) {
     CUTRITON_RETURN_IF_ERROR(add(op, 1, 1, InferLikeFirstInput));
   }
   CUTRITON_RETURN_IF_ERROR(add("LayerNormalization", 2, 3, InferLayerNorm));
   CUTRITON_RETURN_IF_ERROR(add("Add", 2, 2, InferBinary));
   CUTRITON_RETURN_IF_ERROR(add("AddRelu", 2, 2, InferBinary));
+  CUTRITON_RETURN_IF_ERROR(add("Mul", 2, 2, InferBinary));
   CUTRITON_RETURN_IF_ERROR(add("Flatten", 1, 1, InferFlatten));
   CUTRITON_RETURN_IF_ERROR(add("Gemm", 2, 3, InferGemm));
   CUTRITON_RETURN_IF_ERROR(add("GemmGelu", 2, 3, InferGemm));
   CUTRITON_RETURN_IF_ERROR(add("MatMul", 2, 2, InferGemm));
+  CUTRITON_RETURN_IF_ERROR(add("GatedGemm", 3, 3, InferGatedGemm));
+  CUTRITON_RETURN_IF_ERROR(add("QuantizeRows", 1, 1, InferQuantizeRows, 2));
+  CUTRITON_RETURN_IF_ERROR(add("QGemm", 4, 5, InferQGemm));
+  CUTRITON_RETURN_IF_ERROR(add("QGatedGemm", 6, 6, InferQGatedGemm));
   CUTRITON_RETURN_IF_ERROR(add("SkipLayerNormalization", 4, 4, InferSkipLayerNorm));
   CUTRITON_RETURN_IF_ERROR(add("MaxPool", 1, 1, InferPool));
   CUTRITON_RETURN_IF_ERROR(add("AveragePool", 1, 1, InferPool));
@@ -529,6 +692,7 @@ std::unique_ptr<GraphPass> CreateConstantFoldingPass() { return std::make_unique
 std::unique_ptr<GraphPass> CreateDeadNodeEliminationPass() { return std::make_unique<DeadNodeEliminationPass>(); }
 std::unique_ptr<GraphPass> CreateConvBatchNormReluFusionPass() { return std::make_unique<ConvBatchNormReluFusionPass>(); }
 std::unique_ptr<GraphPass> CreateAddReluFusionPass() { return std::make_unique<AddReluFusionPass>(); }
+std::unique_ptr<GraphPass> CreateGatedGemmFusionPass() { return std::make_unique<GatedGemmFusionPass>(); }
 std::unique_ptr<GraphPass> CreateGemmGeluFusionPass() { return std::make_unique<GemmGeluFusionPass>(); }
 std::unique_ptr<GraphPass> CreateSkipLayerNormalizationFusionPass() { return std::make_unique<SkipLayerNormFusionPass>(); }
 std::unique_ptr<GraphPass> CreateFlattenGemmNormalizationPass() { return std::make_unique<FlattenGemmNormalizationPass>(); }
@@ -549,6 +713,8 @@ PassManager CreateCompilePasses(bool enable_transformer_fusions, bool enable_res
   manager.Add(CreateAddReluFusionPass());
   if (enable_residual_fusion) manager.Add(CreateConvResidualFusionPass());
   if (enable_transformer_fusions) {
+    // Before GemmGelu, which would take the gate's GELU away.
+    manager.Add(CreateGatedGemmFusionPass());
     manager.Add(CreateGemmGeluFusionPass());
     manager.Add(CreateSkipLayerNormalizationFusionPass());
   }

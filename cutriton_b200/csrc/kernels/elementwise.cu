@@ -7,7 +7,7 @@
 // Math follows the reference formulas (python/cutriton/triton_kernels/
 // resnet.py:117-156, transformer.py:110-125).
 
-#include "common.cuh"
+#include "product.cuh"
 
 namespace {
 
@@ -69,6 +69,60 @@ __device__ __forceinline__ void binary_f32(const float* __restrict__ a, const fl
   for (long long i = base + threadIdx.x; i < end; i += kThreads) out[i] = op(a[i], b[i]);
 }
 
+// f on FP16 data, computed in FP32, stored round-to-nearest.
+template <typename F>
+__device__ __forceinline__ void unary_f16(const __half* __restrict__ x, __half* __restrict__ out, int total, F f32) {
+  const long long base = static_cast<long long>(blockIdx.x) * kChunkF16;
+  if (base + kChunkF16 <= total && ctb::aligned16(x) && ctb::aligned16(out)) {
+    uint4 v[kVecPerThread];
+#pragma unroll
+    for (int j = 0; j < kVecPerThread; ++j) v[j] = reinterpret_cast<const uint4*>(x + base)[j * kThreads + threadIdx.x];
+#pragma unroll
+    for (int j = 0; j < kVecPerThread; ++j) {
+      __half2* h = reinterpret_cast<__half2*>(&v[j]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = __half22float2(h[k]);
+        h[k] = __floats2half2_rn(f32(f.x), f32(f.y));
+      }
+      reinterpret_cast<uint4*>(out + base)[j * kThreads + threadIdx.x] = v[j];
+    }
+    return;
+  }
+  const long long end = min(static_cast<long long>(total), base + kChunkF16);
+  for (long long i = base + threadIdx.x; i < end; i += kThreads) {
+    out[i] = __float2half_rn(f32(__half2float(x[i])));
+  }
+}
+
+// FP16 operands, f in FP16 arithmetic on pairs.
+template <typename F>
+__device__ __forceinline__ void binary_f16(const __half* __restrict__ a, const __half* __restrict__ b,
+                                           __half* __restrict__ out, int total, F f) {
+  const long long base = static_cast<long long>(blockIdx.x) * kChunkF16;
+  if (base + kChunkF16 <= total && ctb::aligned16(a) && ctb::aligned16(b) && ctb::aligned16(out)) {
+    uint4 va[kVecPerThread], vb[kVecPerThread];
+#pragma unroll
+    for (int j = 0; j < kVecPerThread; ++j) {
+      va[j] = reinterpret_cast<const uint4*>(a + base)[j * kThreads + threadIdx.x];
+      vb[j] = reinterpret_cast<const uint4*>(b + base)[j * kThreads + threadIdx.x];
+    }
+#pragma unroll
+    for (int j = 0; j < kVecPerThread; ++j) {
+      __half2* ha = reinterpret_cast<__half2*>(&va[j]);
+      const __half2* hb = reinterpret_cast<const __half2*>(&vb[j]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) ha[k] = f(ha[k], hb[k]);
+      reinterpret_cast<uint4*>(out + base)[j * kThreads + threadIdx.x] = va[j];
+    }
+    return;
+  }
+  const long long end = min(static_cast<long long>(total), base + kChunkF16);
+  for (long long i = base + threadIdx.x; i < end; i += kThreads) {
+    out[i] = __low2half(f(__half2half2(a[i]), __half2half2(b[i])));
+  }
+}
+
 }  // namespace
 
 extern "C" __global__ void __launch_bounds__(kThreads)
@@ -125,57 +179,33 @@ ctb_batch_norm_f32(const float* x, const float* scale, const float* bias, const 
   }
 }
 
-// Exact-erf GELU on FP16 data, computed in FP32, stored round-to-nearest.
+// Exact-erf GELU.
 extern "C" __global__ void __launch_bounds__(kThreads)
 ctb_gelu_f16(const __half* x, __half* out, int total, CTB_RESERVED_PARAMS) {
   CTB_UNUSED_RESERVED();
   CTB_GRID_DEPENDENCY_SYNC();
-  const long long base = static_cast<long long>(blockIdx.x) * kChunkF16;
-  if (base + kChunkF16 <= total && ctb::aligned16(x) && ctb::aligned16(out)) {
-    uint4 v[kVecPerThread];
-#pragma unroll
-    for (int j = 0; j < kVecPerThread; ++j) v[j] = reinterpret_cast<const uint4*>(x + base)[j * kThreads + threadIdx.x];
-#pragma unroll
-    for (int j = 0; j < kVecPerThread; ++j) {
-      __half2* h = reinterpret_cast<__half2*>(&v[j]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = __half22float2(h[k]);
-        h[k] = __floats2half2_rn(ctb::gelu_erf(f.x), ctb::gelu_erf(f.y));
-      }
-      reinterpret_cast<uint4*>(out + base)[j * kThreads + threadIdx.x] = v[j];
-    }
-    return;
-  }
-  const long long end = min(static_cast<long long>(total), base + kChunkF16);
-  for (long long i = base + threadIdx.x; i < end; i += kThreads) {
-    out[i] = __float2half_rn(ctb::gelu_erf(__half2float(x[i])));
-  }
+  unary_f16(x, out, total, [](float v) { return ctb::gelu_erf(v); });
 }
 
-// FP16 addition in FP16 arithmetic (the unfused Add of the transformer path).
+extern "C" __global__ void __launch_bounds__(kThreads)
+ctb_silu_f16(const __half* x, __half* out, int total, CTB_RESERVED_PARAMS) {
+  CTB_UNUSED_RESERVED();
+  CTB_GRID_DEPENDENCY_SYNC();
+  unary_f16(x, out, total, [](float v) { return ctb::silu(v); });
+}
+
+// FP16 addition and product in FP16 arithmetic (the unfused steps of the
+// transformer path).
 extern "C" __global__ void __launch_bounds__(kThreads)
 ctb_add_f16(const __half* a, const __half* b, __half* out, int total, CTB_RESERVED_PARAMS) {
   CTB_UNUSED_RESERVED();
   CTB_GRID_DEPENDENCY_SYNC();
-  const long long base = static_cast<long long>(blockIdx.x) * kChunkF16;
-  if (base + kChunkF16 <= total && ctb::aligned16(a) && ctb::aligned16(b) && ctb::aligned16(out)) {
-    uint4 va[kVecPerThread], vb[kVecPerThread];
-#pragma unroll
-    for (int j = 0; j < kVecPerThread; ++j) {
-      va[j] = reinterpret_cast<const uint4*>(a + base)[j * kThreads + threadIdx.x];
-      vb[j] = reinterpret_cast<const uint4*>(b + base)[j * kThreads + threadIdx.x];
-    }
-#pragma unroll
-    for (int j = 0; j < kVecPerThread; ++j) {
-      __half2* ha = reinterpret_cast<__half2*>(&va[j]);
-      const __half2* hb = reinterpret_cast<const __half2*>(&vb[j]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) ha[k] = __hadd2(ha[k], hb[k]);
-      reinterpret_cast<uint4*>(out + base)[j * kThreads + threadIdx.x] = va[j];
-    }
-    return;
-  }
-  const long long end = min(static_cast<long long>(total), base + kChunkF16);
-  for (long long i = base + threadIdx.x; i < end; i += kThreads) out[i] = __hadd(a[i], b[i]);
+  binary_f16(a, b, out, total, [](__half2 p, __half2 q) { return __hadd2(p, q); });
+}
+
+extern "C" __global__ void __launch_bounds__(kThreads)
+ctb_mul_f16(const __half* a, const __half* b, __half* out, int total, CTB_RESERVED_PARAMS) {
+  CTB_UNUSED_RESERVED();
+  CTB_GRID_DEPENDENCY_SYNC();
+  binary_f16(a, b, out, total, [](__half2 p, __half2 q) { return __hmul2(p, q); });
 }

@@ -34,7 +34,7 @@ double HalfValue(std::uint16_t bits) {
   return sign * std::ldexp(static_cast<double>(1024 + fraction), exponent - 25);
 }
 
-// Host copy of a tensor's elements as doubles (FP32 / FP16 outputs).
+// Host copy of a tensor's elements as doubles (FP32 / FP16 / 8-bit outputs).
 Status ReadBack(const Tensor& tensor, std::vector<double>* values) {
   const std::size_t count = static_cast<std::size_t>(tensor.desc().NumElements());
   const std::size_t bytes = tensor.desc().ByteSize();
@@ -56,8 +56,11 @@ Status ReadBack(const Tensor& tensor, std::vector<double>* values) {
         (*values)[i] = HalfValue(h);
       }
       return Status::OK();
+    case DataType::kInt8:
+      for (std::size_t i = 0; i < count; ++i) (*values)[i] = static_cast<signed char>(raw[i]);
+      return Status::OK();
     default:
-      return Status::Unsupported("the tuner compares float32 / float16 outputs only");
+      return Status::Unsupported("the tuner compares float32 / float16 / int8 outputs only");
   }
 }
 

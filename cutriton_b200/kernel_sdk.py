@@ -31,7 +31,7 @@ PACK_VERSION = 1
 KERNEL_DIR = Path(__file__).resolve().parent / "csrc" / "kernels"
 
 _SOURCE_FIELDS = {
-    "input": {"kind", "index", "prepack"},
+    "input": {"kind", "index", "prepack", "optional"},
     "output": {"kind", "index"},
     "input_dim": {"kind", "index", "axis"},
     "input_dim_product": {"kind", "index", "begin_axis"},

@@ -265,7 +265,9 @@ def _elementwise_specs() -> list[KernelSpec]:
         ("add.fp32", "Add", "ctb_add_f32", ("a", "b"), "float32", chunk_f32, ""),
         ("add_relu.fp32", "AddRelu", "ctb_add_relu_f32", ("a", "b"), "float32", chunk_f32, ""),
         ("gelu.fp16", "Gelu", "ctb_gelu_f16", ("x",), "float16", chunk_f16, ""),
+        ("silu.fp16", "Silu", "ctb_silu_f16", ("x",), "float16", chunk_f16, ""),
         ("add.fp16", "Add", "ctb_add_f16", ("a", "b"), "float16", chunk_f16, ""),
+        ("mul.fp16", "Mul", "ctb_mul_f16", ("a", "b"), "float16", chunk_f16, ""),
     ):
         ptr = "*fp32" if dtype == "float32" else "*fp16"
         arguments = tuple(arg(n, ptr, "input", index=i) for i, n in enumerate(inputs)) + (
@@ -538,6 +540,65 @@ def _gemm_specs() -> list[KernelSpec]:
     ]
 
 
+# ---- gated and 8-bit products ---------------------------------------------------
+
+PRODUCT_DIMS = (
+    arg("m", "i32", "output_dim", index=0, axis=0),
+    arg("n", "i32", "output_dim", index=0, axis=1),
+    arg("k", "i32", "input_dim", index=0, axis=1),
+)
+ACTIVATION = arg("activation", "i32", "attribute_i64", name="activation", default=0)
+TRANS_B = arg("trans_b", "i32", "attribute_i64", name="transB", default=0)
+HALF_OUT = arg("output", "*fp16", "output", index=0)
+
+# op -> (dtype tag of the kernel id, kernel name, scales and bias in the node's
+# input order, index of each weight matrix)
+PRODUCTS = {
+    "GatedGemm": ("fp16", "gated_gemm", (), (1, 2)),
+    "QGemm": ("i8", "qgemm", (arg("x_scale", "*fp32", "input", index=1), arg("w_scale", "*fp32", "input", index=3),
+                              arg("bias", "*fp16", "input", index=4, optional=1)), (2,)),
+    "QGatedGemm": ("i8", "qgated_gemm", (arg("x_scale", "*fp32", "input", index=1),
+                                         arg("gate_scale", "*fp32", "input", index=3),
+                                         arg("up_scale", "*fp32", "input", index=5)), (2, 4)),
+}
+
+
+def _product_specs() -> list[KernelSpec]:
+    specs = []
+    for op_type, (tag, name, vectors, weights) in PRODUCTS.items():
+        ptr = "*fp16" if tag == "fp16" else "*i8"
+        gated = len(weights) == 2
+        symbol = f"ctb_{name}_{'f16' if tag == 'fp16' else 'i8'}"
+        # Arguments of the general form, in the kernels' order.
+        names = ("w_gate", "w_up") if gated else ("w",)
+        matrices = tuple(arg(n, ptr, "input", index=i) for n, i in zip(names, weights))
+        if tag == "fp16":
+            tensors = matrices
+        elif gated:
+            tensors = (vectors[0], matrices[0], vectors[1], matrices[1], vectors[2])
+        else:
+            tensors = (vectors[0], matrices[0], *vectors[1:])
+        specs.append(KernelSpec(
+            kernel_id=f"{name}.{tag}.any", op_type=op_type, version=1, source="gemm_any.cu", symbol=f"{symbol}_any",
+            arguments=(arg("x", ptr, "input", index=0), *tensors, HALF_OUT, *PRODUCT_DIMS,
+                       *((ACTIVATION,) if gated else ()), TRANS_B) + RESERVED,
+            grid=(ceil_div(out_dim(0), meta("BLOCK_M")), ceil_div(out_dim(1), meta("BLOCK_N"))), dtype="float16",
+            variants=(Variant("m64n64k32", num_warps=8, meta={"BLOCK_M": 64, "BLOCK_N": 64}, default=True),)))
+    # One warp (rows of at most 1024 elements) or one block a row; 16 blocks
+    # an SM cover the block form, whose eight resident ones hide each other's
+    # barriers.
+    specs.append(KernelSpec(
+        kernel_id="quantize_rows.fp16", op_type="QuantizeRows", version=1, source="quantize.cu",
+        symbol="ctb_quantize_rows_f16", dtype="int8",
+        arguments=(arg("x", "*fp16", "input", index=0), arg("q", "*i8", "output", index=0),
+                   arg("scale", "*fp32", "output", index=1), arg("rows", "i32", "input_dim", index=0, axis=0),
+                   arg("columns", "i32", "input_dim", index=0, axis=1)) + RESERVED,
+        grid=({"kind": "min", "args": [{"kind": "input_dim", "index": 0, "axis": 0},
+                                       mul({"kind": "sm_count"}, literal(16))]},),
+        variants=(Variant("row_in_registers", num_warps=8, default=True, programmatic_launch=True),)))
+    return specs
+
+
 def _norm_specs() -> list[KernelSpec]:
     def norm_args(skip: bool) -> tuple[Arg, ...]:
         names = ("x", "residual", "scale", "bias") if skip else ("x", "scale", "bias")
@@ -595,4 +656,5 @@ def _diag_specs() -> list[KernelSpec]:
 
 
 def all_specs() -> list[KernelSpec]:
-    return [*_conv_specs(), *_elementwise_specs(), *_pool_specs(), *_gemm_specs(), *_norm_specs(), *_diag_specs()]
+    return [*_conv_specs(), *_elementwise_specs(), *_pool_specs(), *_gemm_specs(), *_product_specs(), *_norm_specs(),
+            *_diag_specs()]

@@ -61,6 +61,7 @@ struct KernelArgumentSource {
   // it then). swizzle_atom_bytes = 32 (with a 128-byte swizzle) permutes
   // 32-byte instead of 16-byte chunks within each 128-byte row, the layout
   // of MN-major TF32 tensor-core operands.
+  // kInput: an optional input that the node lacks is bound as a null pointer.
   bool map_output{false};
   std::vector<int64_t> box;
   int swizzle_bytes{0};

@@ -21,6 +21,7 @@ enum class DataType {
   kFloat16,
   kInt32,
   kInt64,
+  kInt8,  // sm_100a extension: operands of the 8-bit products
 };
 
 enum class DeviceType {

@@ -38,6 +38,10 @@ std::unique_ptr<GraphPass> CreateDeadNodeEliminationPass();
 std::unique_ptr<GraphPass> CreateConvBatchNormReluFusionPass();
 // Add -> Relu  =>  AddRelu.
 std::unique_ptr<GraphPass> CreateAddReluFusionPass();
+// Gemm -> Silu | Gelu, Mul with a second float16 Gemm of the same input  =>
+// GatedGemm (every value between single-consumer and no graph output).
+// sm_100a extension, part of the transformer fusions.
+std::unique_ptr<GraphPass> CreateGatedGemmFusionPass();
 // Gemm -> Gelu  =>  GemmGelu (Gemm output single-consumer, not a graph output).
 std::unique_ptr<GraphPass> CreateGemmGeluFusionPass();
 // Add -> LayerNormalization  =>  SkipLayerNormalization.
@@ -50,7 +54,7 @@ std::unique_ptr<GraphPass> CreateStaticShapeValidationPass();
 std::unique_ptr<GraphPass> CreateConvResidualFusionPass();
 
 // The reference pipeline: topo, shape, fold, DCE, Conv+BN(+ReLU), Add+ReLU,
-// [GemmGelu, SkipLayerNorm], topo, shape, MatMul/Flatten normalisation, DCE,
+// [GatedGemm, GemmGelu, SkipLayerNorm], topo, shape, MatMul/Flatten normalisation, DCE,
 // validation.
 PassManager CreateDefaultCompilePasses(bool enable_transformer_fusions = true);
 // Same pipeline with the residual epilogue fusion inserted after Add+ReLU.

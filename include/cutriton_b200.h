@@ -35,13 +35,15 @@ typedef enum {
   CTB_INTERNAL = 7
 } ctb_code;
 
-/* Mirrors cutriton::DataType (reference include/cutriton/core/tensor.h:16-22). */
+/* Mirrors cutriton::DataType (reference include/cutriton/core/tensor.h:16-22;
+ * CTB_DTYPE_INT8 is an extension). */
 typedef enum {
   CTB_DTYPE_UNKNOWN = 0,
   CTB_DTYPE_FLOAT32 = 1,
   CTB_DTYPE_FLOAT16 = 2,
   CTB_DTYPE_INT32 = 3,
-  CTB_DTYPE_INT64 = 4
+  CTB_DTYPE_INT64 = 4,
+  CTB_DTYPE_INT8 = 5
 } ctb_dtype;
 
 /* Mirrors cutriton::TuningMode (reference include/cutriton/runtime/tuning.h:7-12). */

@@ -1,0 +1,259 @@
+"""The gated and 8-bit products and the row quantiser on the GPU, every
+candidate against results in 64 bits."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import cutriton_b200 as ct
+import feed_forward_cases as ff
+
+pytestmark = pytest.mark.gpu
+
+
+class Runner:
+    """An engine and a context with CUDA copies of the graph inputs bound; the
+    outputs lie inside larger buffers whose edges must stay as they were."""
+
+    GUARD = 64
+
+    def __init__(self, model, inputs, **options):
+        import torch
+
+        options.setdefault("enable_cuda_graph", False)
+        options.setdefault("tuning_mode", ct.TUNING_DISABLED)
+        self.engine = ct.build_engine(model, **options)
+        self.context = self.engine.create_context()
+        self.inputs = {name: torch.from_numpy(np.ascontiguousarray(a)).cuda() for name, a in inputs.items()}
+        for name, t in self.inputs.items():
+            self.context.bind_tensor(name, t)
+        self.outputs = {}
+        self._whole = {}
+
+    def output(self, name, shape, dtype):
+        import torch
+
+        dtype = getattr(torch, np.dtype(dtype).name)
+        count = int(np.prod(shape))
+        size = torch.empty(0, dtype=dtype).element_size()
+        # 64 guard elements on both sides; 128 bytes keep the middle aligned.
+        guard = max(self.GUARD, 128 // size)
+        whole = torch.full((count + 2 * guard,), 77, dtype=dtype, device="cuda")
+        self._whole[name] = (whole, guard)
+        self.outputs[name] = whole[guard:guard + count].view(shape)
+        self.context.bind_tensor(name, self.outputs[name], output=True)
+
+    def run(self, candidate=None):
+        import torch
+
+        for t in self.outputs.values():
+            t.fill_(77)
+        torch.cuda.synchronize()
+        if candidate is not None:
+            self.context.select_candidate(0, candidate)
+        self.context.run()
+        for name, (whole, guard) in self._whole.items():
+            assert bool((whole[:guard] == 77).all()) and bool((whole[-guard:] == 77).all()), f"{name}: edges written"
+        return {name: t.cpu().numpy() for name, t in self.outputs.items()}
+
+
+def check_product(op, inputs, result, constants=(), **attributes):
+    m, n = result[0].shape
+    runner = Runner(ff.product_graph(op, inputs, constants, **attributes),
+                    {k: v for k, v in inputs.items() if k not in constants})
+    runner.output("y", (m, n), np.float16)
+    ff.assert_within(runner.run()["y"], result, f"{op} default")
+    candidates = runner.engine.op(0)["candidates"]
+    for index, name in enumerate(candidates):
+        try:
+            y = runner.run(index)["y"]
+        except ct.CutritonError as error:
+            # A form for few rows, pinned where it does not apply.
+            assert error.code == ct.SHAPE_ERROR and "stream" in name, (name, error)
+            continue
+        if name.startswith("unfused"):
+            continue  # rounds between its steps; see test_unfused_gated_gemm
+        ff.assert_within(y, result, f"{op} {name}")
+    return candidates
+
+
+# Rows, inner and outer sizes around the tiles of every form: single rows and
+# columns, the row counts where forms change, sizes that end inside a tile, a
+# vector or an 8-element group, and inner sizes of no alignment.
+SIZES = [(1, 8, 1), (1, 16, 8), (1, 1024, 300), (2, 64, 9), (5, 136, 257), (8, 1040, 40), (9, 272, 33), (16, 2048, 129),
+         (17, 80, 64), (31, 512, 100), (33, 144, 200), (64, 4112, 72), (65, 160, 127), (127, 256, 250),
+         (129, 96, 513), (255, 1008, 130), (257, 624, 383), (600, 208, 1000), (3, 7, 5), (70, 33, 90), (130, 1001, 66)]
+
+
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("activation", [ff.SILU, ff.GELU])
+def test_gated_gemm(cuda, size, activation):
+    inputs = ff.gated_case(np.random.default_rng(size), *size)
+    check_product("GatedGemm", inputs, ff.gated_result(inputs, activation), activation=activation, transB=1)
+
+
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("bias", [False, True])
+def test_qgemm(cuda, size, bias):
+    inputs = ff.qgemm_case(np.random.default_rng(size), *size, bias)
+    check_product("QGemm", inputs, ff.qgemm_result(inputs), transB=1)
+
+
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("activation", [ff.SILU, ff.GELU])
+def test_qgated_gemm(cuda, size, activation):
+    inputs = ff.qgated_case(np.random.default_rng(size), *size)
+    check_product("QGatedGemm", inputs, ff.qgated_result(inputs, activation), activation=activation, transB=1)
+
+
+@pytest.mark.parametrize("constant", [False, True])
+@pytest.mark.parametrize("size", [(1, 64, 24), (40, 272, 130), (200, 528, 300)], ids=str)
+def test_weights_by_columns(cuda, size, constant):
+    """transB = 0, the weights as constants and as graph inputs."""
+    rng = np.random.default_rng(7)
+    weights = ("w_gate", "w_up", "w") if constant else ()
+    inputs = ff.gated_case(rng, *size, trans_b=0)
+    check_product("GatedGemm", inputs, ff.gated_result(inputs, 0, trans_b=0), weights)
+    inputs = ff.qgemm_case(rng, *size, True, trans_b=0)
+    check_product("QGemm", inputs, ff.qgemm_result(inputs, trans_b=0), weights)
+    inputs = ff.qgated_case(rng, *size, trans_b=0)
+    check_product("QGatedGemm", inputs, ff.qgated_result(inputs, 1, trans_b=0), weights, activation=1)
+
+
+def test_sums_of_extreme_integers_are_exact(cuda):
+    """All products -128 * -128 = 2^14 over the longest inner dimension: the
+    sum 131056 * 2^14 fits 32 bits, and 2^-31 of it is exact in FP16."""
+    k = 131056
+    for m in (1, 130):
+        x = np.full((m, k), -128, np.int8)
+        w = np.full((40, k), -128, np.int8)
+        w[1::2] = 127
+        inputs = {"x": x, "x_scale": np.full(m, 2.0**-16, np.float32), "w": w,
+                  "w_scale": np.full(40, 2.0**-15, np.float32)}
+        check_product("QGemm", inputs, ff.qgemm_result(inputs), transB=1)
+
+
+def test_large_values_and_non_finite_rows(cuda):
+    """Gates far out on both sides, results beyond FP16 (infinite), rows of
+    NaN and infinity that leave the other rows alone."""
+    rng = np.random.default_rng(3)
+    for m in (6, 200):
+        inputs = ff.gated_case(rng, m, 128, 70)
+        inputs["x"][0] *= np.float16(200)
+        inputs["x"][1, 5] = np.nan
+        inputs["x"][2, 9] = np.inf
+        clean = {**inputs, "x": np.where(np.isfinite(inputs["x"]), inputs["x"], np.float16(0))}
+        for activation in (0, 1):
+            runner = Runner(ff.product_graph("GatedGemm", inputs, activation=activation, transB=1), inputs)
+            runner.output("y", (m, 70), np.float16)
+            expected, tol = ff.gated_result(clean, activation)
+            for index, name in enumerate(runner.engine.op(0)["candidates"]):
+                try:
+                    y = runner.run(index)["y"]
+                except ct.CutritonError as error:
+                    assert error.code == ct.SHAPE_ERROR and "stream" in name
+                    continue
+                assert np.isnan(y[1]).all() and not np.isfinite(y[2]).any(), name
+                over = np.abs(expected) > 65600
+                assert np.isinf(y[0][over[0]]).all(), name
+                inside = (np.abs(expected) < 65000) & ~np.isin(np.arange(m), (1, 2))[:, None]
+                if not name.startswith("unfused"):
+                    assert (np.abs(y.astype(np.float64) - expected) <= tol)[inside].all(), name
+        q = ff.qgemm_case(rng, m, 128, 70, False)
+        q["x_scale"][1], q["x_scale"][2] = np.nan, np.inf
+        q["x"][2] = 0  # what QuantizeRows gives for a row with an infinity
+        runner = Runner(ff.product_graph("QGemm", q, transB=1), q)
+        runner.output("y", (m, 70), np.float16)
+        y = runner.run()["y"]
+        assert np.isnan(y[1]).all() and np.isnan(y[2]).all()
+        assert np.isfinite(y[[0, *range(3, m)]]).all()
+
+
+@pytest.mark.parametrize("activation", [ff.SILU, ff.GELU])
+def test_unfused_gated_gemm(cuda, activation):
+    """The decomposition rounds gate, activation and up projection to FP16
+    too: three more half steps on the product, and theirs on gate and up."""
+    inputs = ff.gated_case(np.random.default_rng(5), 70, 200, 90, trans_b=0)
+    expected, tol = ff.gated_result(inputs, activation, trans_b=0)
+    x = inputs["x"].astype(np.float64)
+    g, u = (np.abs(x @ inputs[w].astype(np.float64)) for w in ("w_gate", "w_up"))
+    tol = tol + ff.HALF * (1.13 * g * u * (1 + ff.HALF) + 3 * np.abs(expected)) + ff.HALF_MIN * (2 * u + 2)
+    runner = Runner(ff.product_graph("GatedGemm", inputs, ("w_gate", "w_up"), activation=activation),
+                    {"x": inputs["x"]})
+    runner.output("y", (70, 90), np.float16)
+    names = runner.engine.op(0)["candidates"]
+    ff.assert_within(runner.run(names.index("unfused:gated_gemm"))["y"], (expected, tol), "unfused")
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (1, 7), (3, 8), (2, 63), (5, 255), (17, 1023), (4, 1024), (9, 1025),
+                                   (1, 4096), (6, 5461), (3, 8192), (2, 8193), (2, 20001), (3000, 40), (2500, 1500)], ids=str)
+def test_quantize_rows(cuda, shape):
+    rng = np.random.default_rng(shape)
+    x = (rng.standard_normal(shape) * np.exp(rng.uniform(-12, 8, (shape[0], 1)))).astype(np.float16)
+    x[rng.integers(0, shape[0])] = 0
+    check_quantize(x)
+
+
+def check_quantize(x, **options):
+    runner = Runner(ff.product_graph("QuantizeRows", {"x": x}), {"x": x}, **options)
+    runner.output("q", x.shape, np.int8)
+    runner.output("q_scale", x.shape[:1], np.float32)
+    got = runner.run()
+    q, scale = ff.quantize_result(x)
+    np.testing.assert_array_equal(got["q_scale"], scale)
+    np.testing.assert_array_equal(got["q"], q)
+
+
+def test_quantize_rows_ties_and_special_values(cuda):
+    """Scales that are powers of two put quotients exactly on halves; FP16's
+    smallest numbers; quotients next to a half; rows of infinity and NaN."""
+    x = np.zeros((40, 300), np.float16)
+    halves = np.arange(-126.5, 127, 1.0)
+    for row in range(20):
+        scale = 2.0 ** (row - 17)
+        x[row, :halves.size] = halves * scale
+        x[row, 299] = 127 * scale
+    x[20, :] = np.float16(2.0**-24) * np.arange(300)
+    x[21, 3] = np.inf
+    x[22, 4] = -np.inf
+    x[23, 5] = np.nan
+    x[24, 6], x[24, 7] = np.nan, np.inf
+    x[25, :] = -0.0
+    x[26, 8] = np.float16(2.0**-24)
+    x[27, :] = 65504
+    rng = np.random.default_rng(0)
+    x[28:] = rng.integers(-2047, 2048, (12, 300)).astype(np.float16)
+    check_quantize(x)
+
+
+def test_quantize_every_half_against_every_scale_step(cuda):
+    """Every finite FP16 magnitude next to 512 different row maxima."""
+    finite = np.arange(0x7C00, dtype=np.uint16).view(np.float16)
+    largest = finite[0x3C00:0x3C00 + 512]  # 1.0 ... 1.5: every mantissa of one binade
+    below = finite[finite <= 1]
+    x = np.concatenate([np.tile(below, (512, 1)), largest[:, None]], axis=1)
+    check_quantize(x)
+
+
+def test_unaligned_tensors(cuda):
+    """Graph inputs and outputs that start one element off every alignment."""
+    import torch
+
+    rng = np.random.default_rng(11)
+    x = rng.standard_normal((5, 2050)).astype(np.float16)
+    engine = ct.build_engine(ff.product_graph("QuantizeRows", {"x": x}), tuning_mode=ct.TUNING_DISABLED)
+    context = engine.create_context()
+    device = torch.zeros(x.size + 1, dtype=torch.float16, device="cuda")
+    device[1:] = torch.from_numpy(x).cuda().reshape(-1)
+    q = torch.full((x.size + 3,), 77, dtype=torch.int8, device="cuda")
+    scale = torch.empty(5, dtype=torch.float32, device="cuda")
+    torch.cuda.synchronize()
+    context.bind_tensor("x", device[1:])
+    context.bind_tensor("q", q[1:x.size + 1], output=True)
+    context.bind_tensor("q_scale", scale, output=True)
+    context.run()
+    want_q, want_scale = ff.quantize_result(x)
+    np.testing.assert_array_equal(q[1:x.size + 1].cpu().numpy().reshape(x.shape), want_q)
+    np.testing.assert_array_equal(scale.cpu().numpy(), want_scale)
+    assert q[0] == 77 and (q[x.size + 1:] == 77).all()
