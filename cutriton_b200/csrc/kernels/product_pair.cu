@@ -1,0 +1,526 @@
+// GatedGemm, QGemm and QGatedGemm on CTA pairs (tcgen05, cta_group::2).
+//
+//   GatedGemm   y = act(x . Wg^T) (x . Wu^T)        FP16 operands, FP32 sums
+//   QGemm       y = (q . W^T) (s[m] ws[n]) + bias   8-bit operands, 32-bit integer sums
+//   QGatedGemm  both
+//
+// with weights [N, K] (a [K, N] constant is turned once at upload), so both
+// operands are K-major rows that TMA brings in blocks of 128 bytes (64 FP16 or
+// 128 8-bit k) in the 128-byte swizzle the tensor core reads; four MMAs of 32
+// bytes of k each use a block up.
+//
+// Two CTAs of a cluster (two SMs) work on one tile of 256 rows: CTA r holds
+// rows 128 r ... of x and half of the BN weight rows, and one
+// tcgen05.mma.cta_group::2 (M = 256, N = BN) reads both halves and leaves 128
+// rows of sums in each CTA's TMEM. For the gated ops the halves are the same
+// BN / 2 columns of the two weight matrices: CTA 0 loads gate rows, CTA 1 up
+// rows, and columns c and BN / 2 + c of every TMEM lane are the gate and the
+// up sum of one output, so activation and product are the epilogue of the
+// thread that reads them and neither projection ever leaves the SM.
+//
+// Warp 0 loads (a ring of 192 KB), warp 1 of CTA 0 issues the MMAs into one of
+// two accumulators, 16 epilogue warps of each CTA turn the other one into
+// FP16 through 32 x 32 boxes that TMA stores. Tiles go round the pairs in
+// blocks of kRasterRows tile rows, so that the 74 pairs at work share about
+// 8 + 9 operand tiles in L2 instead of streaming all weights past each row of
+// tiles. All waits are bounded (tc_common.cuh).
+
+#include "product.cuh"
+#include "tc_common.cuh"
+
+namespace {
+
+using namespace ctb::tc;
+
+constexpr int kBM = 128;  // rows a CTA (the pair covers 256)
+constexpr int kRowBytes = 128;
+constexpr int kEpilogueWarps = 16;
+constexpr int kThreads = (2 + kEpilogueWarps) * 32;
+constexpr int kChunk = 32;
+constexpr int kEpilogueWarp0 = 2;
+constexpr int kRasterRows = 8;
+constexpr uint32_t kTileA = kBM * kRowBytes;  // 16 KB
+constexpr uint32_t kRingBytes = 196608;
+constexpr uint32_t kStageBoxBytes = 32 * kChunk * 2;
+constexpr uint32_t kStagingBytes = kEpilogueWarps * kStageBoxBytes;
+constexpr int kMaxStages = 9;
+constexpr int kSmallBox = 32;  // weight rows of the small box; the large one has 128
+
+struct Half {
+  static constexpr int kBlock = 64;  // k of a 128-byte row
+  // FP16 operands, FP32 sums.
+  static __host__ __device__ constexpr uint32_t idesc(uint32_t m, uint32_t n) { return instr_desc(kFormatF16, m, n); }
+};
+struct Int8 {
+  static constexpr int kBlock = 128;
+  // Signed 8-bit operands (format 1), 32-bit integer sums (D format 2).
+  static __host__ __device__ constexpr uint32_t idesc(uint32_t m, uint32_t n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
+  }
+};
+
+template <int BN, bool kGated>
+struct Shape {
+  static constexpr int kHalf = BN / 2;                      // weight rows a CTA
+  static constexpr int kColumns = kGated ? BN / 2 : BN;     // output columns a tile
+  static constexpr uint32_t kTileB = kHalf * kRowBytes;
+  static constexpr uint32_t kStageBytes = kTileA + kTileB;  // both multiples of 1024
+  static constexpr int kStages = kRingBytes / kStageBytes;
+  static constexpr uint32_t kTmemCols = 2 * BN <= 128 ? 128 : 2 * BN <= 256 ? 256 : 512;
+  static constexpr int kChunks = kColumns / kChunk;
+  static constexpr int kActive = kChunks < kEpilogueWarps / 4 ? kChunks : kEpilogueWarps / 4;  // warps a lane quarter
+  static_assert(kStages <= kMaxStages && kHalf % kSmallBox == 0 && kColumns % kChunk == 0, "tile");
+};
+
+struct __align__(8) Barriers {
+  uint64_t full[kMaxStages];   // leader: both CTAs' copies of a stage landed
+  uint64_t empty[kMaxStages];  // each CTA: the stage's MMAs are done
+  uint64_t tmem_full[2];       // each CTA: the accumulator is complete
+  uint64_t tmem_empty[2];      // leader: the pair's epilogue warps have read it
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+  int consumed;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_addr(const void* local, uint32_t rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(local)), "r"(rank));
+  return remote;
+}
+
+// Tile load into this CTA's shared memory that counts on the leader's barrier.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const TmaDescriptor* desc, uint32_t leader_bar, int x,
+                                                 int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(desc)), "r"(leader_bar), "r"(x), "r"(y)
+      : "memory");
+}
+
+// Arrives on `bar` in both CTAs when this thread's earlier MMAs are done.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  const uint32_t peer = cluster_addr(bar, 1);
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+               : "memory");
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(peer) : "memory");
+}
+
+__device__ __forceinline__ void umma_pair(Half, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void umma_pair(Int8, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void arrive_on_leader(uint64_t* bar) {
+  const uint32_t remote = cluster_addr(bar, 0);
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+}
+
+__device__ __forceinline__ void tma_store_2d(const TmaDescriptor* desc, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(desc)),
+               "r"(smem_addr(src)), "r"(x), "r"(y)
+               : "memory");
+}
+
+// Two 32 x 32 blocks of sums in one wait: 32 columns from `a` and 32 from `b`.
+__device__ __forceinline__ void tmem_load_two(uint32_t a, uint32_t b, uint32_t (&v)[32], uint32_t (&u)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20,"
+      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50,"
+      "%51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]),
+        "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+        "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(a), "r"(b)
+      : "memory");
+}
+
+// What the kernels bind. Weight operand o arrives through boxes of 128 or of
+// kSmallBox rows. Scales are null in FP16.
+struct Operands {
+  const TmaDescriptor* x;
+  const TmaDescriptor* w[2][2];  // [gate / up][large box, small box]
+  const TmaDescriptor* out_map;
+  __half* out;
+  const float* x_scale;
+  const float* w_scale[2];
+  const __half* bias;
+  int m, n, k, activation;
+  void* scratch;
+};
+
+// Tile `index` in raster order: blocks of kRasterRows tile rows, within a
+// block column by column.
+__device__ __forceinline__ void tile_at(int index, int m_tiles, int n_tiles, int* mt, int* nt) {
+  const int per_block = kRasterRows * n_tiles;
+  const int block = index / per_block;
+  const int rows = min(kRasterRows, m_tiles - block * kRasterRows);
+  const int in_block = index - block * per_block;
+  *nt = in_block / rows;
+  *mt = block * kRasterRows + in_block - *nt * rows;
+}
+
+// One lane's 32 outputs of a chunk: `v` the (gate) sums, `u` the up sums.
+template <typename T, bool kGated>
+__device__ __forceinline__ void finish(const Operands& op, uint32_t (&v)[kChunk], uint32_t (&u)[kChunk], int column0,
+                                       float row_scale, uint4 (&packed)[kChunk / 8]) {
+  constexpr bool kInt8 = T::kBlock == 128;
+  const int lane = threadIdx.x & 31;
+  float y[kChunk];
+  if constexpr (kInt8) {
+    const int column = min(column0 + lane, op.n - 1);
+    // A lane is a row: it gets the columns' scales from the lanes that loaded them.
+    const float c0 = __ldg(op.w_scale[0] + column);
+    const float c1 = kGated ? __ldg(op.w_scale[1] + column) : 0.0f;
+    const float bias = !kGated && op.bias != nullptr ? __half2float(op.bias[column]) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      const float s0 = __shfl_sync(0xFFFFFFFFu, c0, j);
+      const float b = kGated ? 0.0f : __shfl_sync(0xFFFFFFFFu, bias, j);
+      y[j] = ctb::dequantized(static_cast<int>(v[j]), row_scale, s0, b);
+      if (kGated) {
+        const float s1 = __shfl_sync(0xFFFFFFFFu, c1, j);
+        u[j] = __float_as_uint(ctb::dequantized(static_cast<int>(u[j]), row_scale, s1, 0.0f));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) y[j] = __uint_as_float(v[j]);
+  }
+  if constexpr (kGated) {
+    if (op.activation == ctb::kSilu) {
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) y[j] = ctb::silu_fast(y[j]) * __uint_as_float(u[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) y[j] = ctb::gelu_erf_fast(y[j]) * __uint_as_float(u[j]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kChunk / 8; ++i) {
+    __half2* h = reinterpret_cast<__half2*>(&packed[i]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(y[8 * i + 2 * j], y[8 * i + 2 * j + 1]);
+  }
+}
+
+template <typename T, bool kGated, int BN>
+__device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op) {
+  using S = Shape<BN, kGated>;
+  constexpr int kStages = S::kStages;
+  uint8_t* staging = smem + kRingBytes;
+  Barriers* bars = reinterpret_cast<Barriers*>(staging + kStagingBytes);
+  volatile int* abort = &bars->abort;
+  auto tile_a = [&](int s) { return smem + s * S::kStageBytes; };
+  auto tile_b = [&](int s) { return smem + s * S::kStageBytes + kTileA; };
+
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  const int pairs = gridDim.x / 2;
+  const int pair = blockIdx.x / 2;
+  const int k_blocks = (op.k + T::kBlock - 1) / T::kBlock;
+  const int n_tiles = (op.n + S::kColumns - 1) / S::kColumns;
+  const int m_tiles = (op.m + 2 * kBM - 1) / (2 * kBM);
+  const int tiles = m_tiles * n_tiles;
+  const int my_tiles = tiles > pair ? (tiles - 1 - pair) / pairs + 1 : 0;
+  const bool tma_epilogue = op.n % 8 == 0 && ctb::aligned16(op.out);
+  constexpr int kBox = BN == 256 ? 0 : 1;
+  const TmaDescriptor* my_w = kGated && !leader ? op.w[1][kBox] : op.w[0][kBox];
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bars->tmem_full[b], 1);
+      mbar_init(&bars->tmem_empty[b], 2 * 4 * S::kActive);
+    }
+    mbar_init(&bars->drain, 1);
+    bars->abort = 0;
+    bars->consumed = 0;
+    mbar_init_fence();
+    tma_prefetch(op.x);
+    tma_prefetch(my_w);
+    if (tma_epilogue) tma_prefetch(op.out_map);
+  }
+  // The peer's copies and commits reach these barriers: both CTAs have
+  // initialised them before either goes on.
+  cluster_sync();
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&bars->tmem_base)),
+                 "r"(S::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = bars->tmem_base;
+  CTB_GRID_DEPENDENCY_SYNC();
+
+  if (warp == 0 && lane == 0) {
+    // ---- TMA producer: this CTA's rows of x and of the weights ----
+    int g = 0;
+    bool stop = false;
+    for (int local = 0; local < my_tiles && !stop; ++local) {
+      int mt, nt;
+      tile_at(pair + local * pairs, m_tiles, n_tiles, &mt, &nt);
+      const int m0 = mt * 2 * kBM + static_cast<int>(rank) * kBM;
+      const int n0 = nt * S::kColumns + (kGated ? 0 : static_cast<int>(rank) * S::kHalf);
+      for (int kb = 0; kb < k_blocks; ++kb, ++g) {
+        const int s = g % kStages;
+        const int use = g / kStages;
+        if (use > 0 && !mbar_wait(&bars->empty[s], (use - 1) & 1, abort, op.scratch, 70)) {
+          stop = true;
+          break;
+        }
+        if (leader) mbar_arrive_expect_tx(&bars->full[s], 2 * S::kStageBytes);
+        const uint32_t full_on_leader = cluster_addr(&bars->full[s], 0);
+        tma_load_2d_pair(tile_a(s), op.x, full_on_leader, kb * T::kBlock, m0);
+        if constexpr (BN == 256) {
+          tma_load_2d_pair(tile_b(s), my_w, full_on_leader, kb * T::kBlock, n0);
+        } else {
+#pragma unroll
+          for (int r = 0; r < S::kHalf; r += kSmallBox) {
+            tma_load_2d_pair(tile_b(s) + r * kRowBytes, my_w, full_on_leader, kb * T::kBlock, n0 + r);
+          }
+        }
+      }
+    }
+    if (*abort && leader) {
+      // Let the issued copies land before shared memory is released (the
+      // peer's too: the leader's barrier counts them). Bounded: a phase the
+      // aborted peer never fed times out after the wait limit.
+      for (int q = *reinterpret_cast<volatile int*>(&bars->consumed); q < g; ++q) {
+        volatile int never = 0;
+        mbar_wait(&bars->full[q % kStages], (q / kStages) & 1, &never, op.scratch, 71);
+      }
+    }
+  } else if (warp == 1 && lane == 0 && leader) {
+    // ---- MMA issuer (pair leader) ----
+    constexpr uint32_t idesc = T::idesc(2 * kBM, BN);
+    int g = 0;
+    bool ok = true;
+    for (int local = 0; local < my_tiles && ok; ++local) {
+      const int buf = local & 1;
+      if (local >= 2 && !mbar_wait(&bars->tmem_empty[buf], ((local >> 1) - 1) & 1, abort, op.scratch, 72)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after_sync();
+      const uint32_t acc = tmem + buf * BN;
+      for (int kb = 0; kb < k_blocks; ++kb, ++g) {
+        const int s = g % kStages;
+        if (!mbar_wait(&bars->full[s], (g / kStages) & 1, abort, op.scratch, 73)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint64_t a_desc = smem_desc_kmajor_sw128(tile_a(s));
+        const uint64_t b_desc = smem_desc_kmajor_sw128(tile_b(s));
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          umma_pair(T{}, acc, a_desc + 2 * kk, b_desc + 2 * kk, idesc, (kb | kk) != 0);
+        }
+        umma_commit_pair(&bars->empty[s]);
+        *reinterpret_cast<volatile int*>(&bars->consumed) = g + 1;
+      }
+      if (ok) umma_commit_pair(&bars->tmem_full[buf]);
+    }
+    if (!ok) {
+      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                       smem_addr(&bars->drain))
+                   : "memory");
+      volatile int never = 0;
+      mbar_wait(&bars->drain, 0, &never, op.scratch, 74);
+    }
+  } else if (warp >= kEpilogueWarp0 && (warp - kEpilogueWarp0) / 4 < S::kActive) {
+    // ---- epilogue: this CTA's 128 rows, quarter = warp % 4 ----
+    const int quarter = warp & 3;
+    const int wq = (warp - kEpilogueWarp0) / 4;
+    uint8_t* box_smem = staging + (warp - kEpilogueWarp0) * kStageBoxBytes;
+    bool box_used = false;
+    for (int local = 0; local < my_tiles; ++local) {
+      const int buf = local & 1;
+      int mt, nt;
+      tile_at(pair + local * pairs, m_tiles, n_tiles, &mt, &nt);
+      const int row0 = mt * 2 * kBM + static_cast<int>(rank) * kBM + quarter * 32;
+      const int n0 = nt * S::kColumns;
+      const float row_scale = op.x_scale != nullptr && row0 + lane < op.m ? __ldg(op.x_scale + row0 + lane) : 0.0f;
+      const bool ready = mbar_wait(&bars->tmem_full[buf], (local >> 1) & 1, abort, op.scratch, 75);
+      __syncwarp();
+      if (!ready) break;
+      tc_fence_after_sync();
+      const uint32_t taddr = tmem + buf * BN + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll 1
+      for (int ci = wq; ci < S::kChunks; ci += S::kActive) {
+        const int c = ci * kChunk;
+        uint32_t v[kChunk], u[kChunk];
+        if constexpr (kGated) {
+          tmem_load_two(taddr + c, taddr + S::kHalf + c, v, u);
+        } else {
+          tmem_load_32x32(taddr + c, v);
+        }
+        if (ci + S::kActive >= S::kChunks) {
+          // This warp's columns are in registers: release them to the issuer.
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            if (leader) {
+              mbar_arrive(&bars->tmem_empty[buf]);
+            } else {
+              arrive_on_leader(&bars->tmem_empty[buf]);
+            }
+          }
+        }
+        // Columns past N (a partial last tile) and rows past M: nothing to store.
+        if (n0 + c >= op.n || row0 >= op.m) continue;
+        uint4 packed[kChunk / 8];
+        finish<T, kGated>(op, v, u, n0 + c, row_scale, packed);
+        if (box_used) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+        }
+        // Row `lane` (64 bytes); 64-byte swizzle: 16-byte chunk i at i ^ ((lane / 2) % 4).
+#pragma unroll
+        for (int i = 0; i < kChunk / 8; ++i) {
+          *reinterpret_cast<uint4*>(box_smem + lane * 64 + (((i ^ (lane >> 1)) & 3) << 4)) = packed[i];
+        }
+        if (tma_epilogue) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(op.out_map, box_smem, n0 + c, row0);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          box_used = true;
+        } else {
+          // Rows that TMA cannot address (N no multiple of 8, an output off
+          // 16 bytes): one row of 32 columns a store instruction.
+          __syncwarp();
+          const int column = n0 + c + lane;
+#pragma unroll 4
+          for (int r = 0; r < 32 && row0 + r < op.m; ++r) {
+            const __half h = *reinterpret_cast<const __half*>(
+                box_smem + r * 64 + ((((lane >> 3) ^ (r >> 1)) & 3) << 4) + (lane & 7) * 2);
+            if (column < op.n) op.out[static_cast<long long>(row0 + r) * op.n + column] = h;
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  // Neither CTA leaves (or frees TMEM) while its peer may still signal it.
+  cluster_sync();
+  tc_fence_after_sync();
+  if (warp == 0) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kTmemCols) : "memory");
+  }
+}
+
+// Tile width: the least waves of pair tiles times a tile's cost. Both CTAs of
+// a pair compute it from the same arguments, so they agree.
+template <typename T, bool kGated>
+__device__ __forceinline__ void product_dispatch(const Operands& op) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+  const long long m_tiles = (op.m + 2 * kBM - 1) / (2 * kBM);
+  const long long pairs = gridDim.x / 2;
+  const auto cost = [&](int bn, int tile_cost) {
+    const int columns = kGated ? bn / 2 : bn;
+    const long long tiles = m_tiles * ((op.n + columns - 1) / columns);
+    return (tiles + pairs - 1) / pairs * tile_cost;
+  };
+  const long long t256 = cost(256, 100), t192 = cost(192, 80), t128 = cost(128, 62), t64 = cost(64, 45);
+  const long long best = min(min(t256, t192), min(t128, t64));
+  if (t256 == best) {
+    product_pair<T, kGated, 256>(smem, op);
+  } else if (t192 == best) {
+    product_pair<T, kGated, 192>(smem, op);
+  } else if (t128 == best) {
+    product_pair<T, kGated, 128>(smem, op);
+  } else {
+    product_pair<T, kGated, 64>(smem, op);
+  }
+}
+
+}  // namespace
+
+extern "C" __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+ctb_gated_gemm_f16_pair(const __grid_constant__ TmaDescriptor tma_x, const __grid_constant__ TmaDescriptor tma_gate128,
+                        const __grid_constant__ TmaDescriptor tma_gate32,
+                        const __grid_constant__ TmaDescriptor tma_up128, const __grid_constant__ TmaDescriptor tma_up32,
+                        const __grid_constant__ TmaDescriptor tma_out, __half* output, int m, int n, int k,
+                        int activation, CTB_RESERVED_PARAMS) {
+  (void)profile_scratch;
+  const Operands op = {&tma_x,  {{&tma_gate128, &tma_gate32}, {&tma_up128, &tma_up32}},
+                       &tma_out, output, nullptr, {nullptr, nullptr}, nullptr, m, n, k, activation, runtime_scratch};
+  product_dispatch<Half, true>(op);
+}
+
+extern "C" __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+ctb_qgemm_i8_pair(const __grid_constant__ TmaDescriptor tma_x, const __grid_constant__ TmaDescriptor tma_w128,
+                  const __grid_constant__ TmaDescriptor tma_w32, const __grid_constant__ TmaDescriptor tma_out,
+                  const float* x_scale, const float* w_scale, const __half* bias, __half* output, int m, int n, int k,
+                  CTB_RESERVED_PARAMS) {
+  (void)profile_scratch;
+  const Operands op = {&tma_x,  {{&tma_w128, &tma_w32}, {nullptr, nullptr}},
+                       &tma_out, output, x_scale, {w_scale, nullptr}, bias, m, n, k, 0, runtime_scratch};
+  product_dispatch<Int8, false>(op);
+}
+
+extern "C" __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+ctb_qgated_gemm_i8_pair(const __grid_constant__ TmaDescriptor tma_x, const __grid_constant__ TmaDescriptor tma_gate128,
+                        const __grid_constant__ TmaDescriptor tma_gate32,
+                        const __grid_constant__ TmaDescriptor tma_up128, const __grid_constant__ TmaDescriptor tma_up32,
+                        const __grid_constant__ TmaDescriptor tma_out, const float* x_scale, const float* gate_scale,
+                        const float* up_scale, __half* output, int m, int n, int k, int activation,
+                        CTB_RESERVED_PARAMS) {
+  (void)profile_scratch;
+  const Operands op = {&tma_x,  {{&tma_gate128, &tma_gate32}, {&tma_up128, &tma_up32}},
+                       &tma_out, output, x_scale, {gate_scale, up_scale}, nullptr, m, n, k, activation,
+                       runtime_scratch};
+  product_dispatch<Int8, true>(op);
+}

@@ -583,7 +583,35 @@ def _product_specs() -> list[KernelSpec]:
             arguments=(arg("x", ptr, "input", index=0), *tensors, HALF_OUT, *PRODUCT_DIMS,
                        *((ACTIVATION,) if gated else ()), TRANS_B) + RESERVED,
             grid=(ceil_div(out_dim(0), meta("BLOCK_M")), ceil_div(out_dim(1), meta("BLOCK_N"))), dtype="float16",
-            variants=(Variant("m64n64k32", num_warps=8, meta={"BLOCK_M": 64, "BLOCK_N": 64}, default=True),)))
+            variants=(Variant("m64n64k32", num_warps=8, meta={"BLOCK_M": 64, "BLOCK_N": 64}),)))
+        # CTA pairs: boxes are rows of 128 bytes; one variant for weights
+        # given by output channel, one that turns a [K, N] constant at upload.
+        block = 64 if tag == "fp16" else 128
+        maps = [arg("tma_x", "tensormap", "tensor_map", tensor="input", index=0, box=[block, 128], swizzle=128)]
+        for n, i in zip(("gate", "up") if gated else ("w",), weights):
+            maps += [arg(f"tma_{n}{rows}", "tensormap", "tensor_map", tensor="input", index=i, box=[block, rows],
+                         swizzle=128) for rows in (128, 32)]
+        maps.append(arg("tma_out", "tensormap", "tensor_map", tensor="output", index=0, box=[32, 32], swizzle=64,
+                        optional=1))
+        turned = {a.name: {"prepack": "transpose_2d"} for a in maps[1:-1]}
+        columns = 32 if gated else 64  # of the narrowest tile
+        rows_of_16_bytes = {"kind": "dim_multiple_of", "source": "input", "index": 0, "axis": 1,
+                            "value": 8 if tag == "fp16" else 16}
+        pair = dict(num_warps=18, shared_memory_bytes=196608 + 32768 + 256 + 1024, programmatic_launch=True)
+        by_rows = {"kind": "attribute_i64_eq", "name": "transB", "value": 1, "default": 0}
+        by_columns = {"kind": "attribute_i64_eq", "name": "transB", "value": 0, "default": 0}
+        specs.append(KernelSpec(
+            kernel_id=f"{name}.{tag}.pair", op_type=op_type, version=1, source="product_pair.cu",
+            symbol=f"{symbol}_pair",
+            arguments=(*maps, *vectors, HALF_OUT, *PRODUCT_DIMS, *((ACTIVATION,) if gated else ())) + RESERVED,
+            grid=(mul(literal(2), {"kind": "min", "args": [
+                mul(ceil_div(out_dim(0), literal(256)), ceil_div(out_dim(1), literal(columns))),
+                ceil_div({"kind": "sm_count"}, literal(2))]}),),
+            dtype="float16", constraints=(rows_of_16_bytes,),
+            variants=(Variant("m256k128b", default=True, constraints=(by_rows,), **pair),
+                      Variant("m256k128b_turned", arg_overrides=turned,
+                              constraints=(by_columns, *({"kind": "input_is_constant", "index": i} for i in weights)),
+                              **pair))))
     # One warp (rows of at most 1024 elements) or one block a row; 16 blocks
     # an SM cover the block form, whose eight resident ones hide each other's
     # barriers.
