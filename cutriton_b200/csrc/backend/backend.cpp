@@ -151,6 +151,7 @@ std::string VariantProblem(const KernelArtifact& artifact, const Node& node, con
     if (v == nullptr || !v->is_constant) return "prepacks argument '" + argument.name + "', which is not a constant";
   }
   for (std::size_t i = 0; i < artifact.constraints.size(); ++i) {
+    if (artifact.constraints[i].at_run) continue;  // the context's choice, at each run's shapes
     if (!ConstraintHolds(artifact.constraints[i], node, lookup)) return "constraint " + std::to_string(i) + " fails";
   }
   return "";
@@ -221,6 +222,10 @@ const KernelArtifact* PickSubKernel(const ArtifactRepository& repository, const 
   const KernelArtifact* fallback = nullptr;
   for (const auto& a : *list) {
     if (a.dtype != dtype || !ArtifactMatches(a, sub, lookup, capability)) continue;
+    // A step's kernel is fixed here, for every shape of the plan.
+    if (std::any_of(a.constraints.begin(), a.constraints.end(), [](const KernelConstraint& c) { return c.at_run; })) {
+      continue;
+    }
     if (a.is_default) return &a;
     if (sibling == nullptr && a.kernel_id == default_kernel) sibling = &a;
     if (fallback == nullptr) fallback = &a;
@@ -463,6 +468,22 @@ Status RegisterBuiltinBackends() {
   CUTRITON_RETURN_IF_ERROR(RegisterIfMissing(CreateCpuReferenceBackend()));
   CUTRITON_RETURN_IF_ERROR(RegisterIfMissing(CreateCudaSm100Backend()));
   return Status::OK();
+}
+
+bool HoldsAtRun(const ExecutionCandidate& candidate, const Node& node, const Graph& graph, bool* any) {
+  const ValueLookup lookup = [&](const std::string& n) { return graph.FindValue(n); };
+  bool holds = true;
+  if (any != nullptr) *any = false;
+  for (const PlanStep& step : candidate.steps) {
+    const auto* kernel = std::get_if<KernelInvocation>(&step);
+    if (kernel == nullptr) continue;
+    for (const KernelConstraint& c : kernel->artifact.constraints) {
+      if (!c.at_run) continue;
+      if (any != nullptr) *any = true;
+      holds = holds && ConstraintHolds(c, node, lookup);
+    }
+  }
+  return holds;
 }
 
 bool IsCudaArtifactTarget(const std::string& target) {

@@ -251,6 +251,7 @@ KernelConstraint ParseConstraint(const json::Value& v) {
     c.axis = AsInt(v.at("axis"));
     c.expected = AsInt(v.at("value"));
     if (c.expected <= 0) throw std::runtime_error(kind + " value must be positive");
+    c.at_run = IntOr(v, "at_run", 0) != 0;
   } else if (kind == "input_is_constant") {
     c.kind = KernelConstraintKind::kInputIsConstant;
     c.tensor_index = AsInt(v.at("index"));

@@ -201,6 +201,31 @@ Status CheckBinding(const std::string& name, const TensorDesc& want, const Tenso
   return Status::OK();
 }
 
+// The candidate `op` runs at the shapes of `graph`: the pinned one; else the
+// first whose run-time constraints (it has some) hold; else the default of the
+// lowering. `admitted` tells for each candidate whether it takes the shapes.
+Status ChooseCandidate(const PlanOp& op, const Graph& graph, const std::size_t* pin, std::size_t* chosen,
+                       std::vector<char>* admitted) {
+  const Node& node = graph.nodes().at(static_cast<std::size_t>(op.node_id));
+  admitted->assign(op.candidates.size(), 1);
+  *chosen = op.selected_candidate;
+  bool found = false;
+  for (std::size_t c = 0; c < op.candidates.size(); ++c) {
+    bool any = false;
+    (*admitted)[c] = HoldsAtRun(op.candidates[c], node, graph, &any);
+    if (any && (*admitted)[c] && !found) {
+      *chosen = c;
+      found = true;
+    }
+  }
+  if (pin != nullptr) *chosen = *pin;
+  if (*chosen < op.candidates.size() && !(*admitted)[*chosen]) {
+    return Status::ShapeError("op " + op.node_name + ": candidate " + op.candidates[*chosen].candidate_id +
+                              " does not take this run's shapes");
+  }
+  return Status::OK();
+}
+
 bool OnlyViews(const ExecutionCandidate& candidate) {
   return std::none_of(candidate.steps.begin(), candidate.steps.end(),
                       [](const PlanStep& s) { return std::holds_alternative<KernelInvocation>(s); });
@@ -450,9 +475,11 @@ Status ExecutionContext::PrepareTuning() {
   if (s.selection_at == std::make_pair(s.layout, s.choice)) return Status::OK();
   const auto& ops = state_->plan.ops();
   std::vector<std::size_t> chosen(ops.size());
+  std::vector<std::vector<char>> admitted(ops.size());
   for (std::size_t i = 0; i < ops.size(); ++i) {
     const auto pin = s.pins.find(i);
-    chosen[i] = pin != s.pins.end() ? pin->second : ops[i].selected_candidate;
+    CUTRITON_RETURN_IF_ERROR(
+        ChooseCandidate(ops[i], ActiveGraph(), pin == s.pins.end() ? nullptr : &pin->second, &chosen[i], &admitted[i]));
   }
   const TuningConfig& config = state_->plan.tuning_config();
   if (state_->on_cuda() && config.mode != TuningMode::kDisabled) {
@@ -479,7 +506,7 @@ Status ExecutionContext::PrepareTuning() {
       if (cached) {
         const auto match = std::find_if(op.candidates.begin(), op.candidates.end(),
                                         [&](const ExecutionCandidate& c) { return c.candidate_id == *cached; });
-        if (match != op.candidates.end()) {
+        if (match != op.candidates.end() && admitted[i][static_cast<std::size_t>(match - op.candidates.begin())]) {
           chosen[i] = static_cast<std::size_t>(match - op.candidates.begin());
           continue;
         }
@@ -493,6 +520,8 @@ Status ExecutionContext::PrepareTuning() {
       target.error_word = s.device == nullptr ? nullptr : s.device->error_word_device();
       if (s.device != nullptr) target.take_device_error = [&s] { return s.device->TakeDeviceError(); };
       target.modules = modules;
+      target.fallback = chosen[i];
+      target.admitted = admitted[i];
       std::vector<double> medians;
       CUTRITON_RETURN_IF_ERROR(runtime::TuneCandidates(target, config, &chosen[i], &medians));
       CUTRITON_RETURN_IF_ERROR(runtime::StoreTuningChoice(config.cache_dir, key, op, chosen[i], medians));

@@ -245,7 +245,7 @@ Status TuneCandidates(const TuningTarget& target, const TuningConfig& config, st
   const double tolerance = output.desc().dtype == DataType::kFloat16 ? 1e-2 : 1e-4;
 
   // Warm-up and eligibility, default candidate first (it is the reference).
-  const std::size_t fallback = op.selected_candidate;
+  const std::size_t fallback = target.fallback;
   std::vector<std::size_t> eligible;
   std::vector<double> reference;
   std::vector<std::size_t> order{fallback};
@@ -253,7 +253,7 @@ Status TuneCandidates(const TuningTarget& target, const TuningConfig& config, st
     if (c != fallback) order.push_back(c);
   }
   for (std::size_t c : order) {
-    if (kernels[c].empty()) continue;
+    if (kernels[c].empty() || !target.admitted[c]) continue;
     for (int w = 0; w < std::max(1, config.warmup_iterations); ++w) CUTRITON_RETURN_IF_ERROR(launch(c));
     CUTRITON_RETURN_IF_ERROR(drv::Check(api.cuStreamSynchronize(timer.stream), "cuStreamSynchronize"));
     // A candidate whose kernel reported an error (a shape or alignment

@@ -49,6 +49,10 @@ struct TuningTarget {
   // status means a kernel of the candidate just run reported an error.
   std::function<Status()> take_device_error;
   std::shared_ptr<CudaModuleCache> modules;
+  // The candidate to keep unless another is faster, and which of them take
+  // this run's shapes.
+  std::size_t fallback{0};
+  std::vector<char> admitted;
 };
 
 // Picks the candidate of `target.op` to run; `median_ms` gets one entry per

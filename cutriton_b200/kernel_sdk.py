@@ -49,8 +49,8 @@ _CONSTRAINT_FIELDS = {
     "input_count_eq": {"kind", "value"},
     "tensor_rank_eq": {"kind", "source", "index", "value"},
     "attribute_list_eq": {"kind", "name", "value", "default"},
-    "dim_multiple_of": {"kind", "source", "index", "axis", "value"},
-    "dim_le": {"kind", "source", "index", "axis", "value"},
+    "dim_multiple_of": {"kind", "source", "index", "axis", "value", "at_run"},
+    "dim_le": {"kind", "source", "index", "axis", "value", "at_run"},
     "input_is_constant": {"kind", "index"},
 }
 _GRID_FIELDS = {

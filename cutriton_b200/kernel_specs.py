@@ -612,6 +612,23 @@ def _product_specs() -> list[KernelSpec]:
                       Variant("m256k128b_turned", arg_overrides=turned,
                               constraints=(by_columns, *({"kind": "input_is_constant", "index": i} for i in weights)),
                               **pair))))
+        # Few rows, weights by output channel: chosen at run time, as M is what
+        # shape profiles leave open.
+        stream = dict(num_warps=8, shared_memory_bytes=229376, programmatic_launch=True)
+        few_rows = {"kind": "dim_le", "source": "input", "index": 0, "axis": 0, "value": 32, "at_run": 1}
+        stream_turned = {a.name: {"prepack": "transpose_2d"} for a in matrices}
+        specs.append(KernelSpec(
+            kernel_id=f"{name}.{tag}.stream", op_type=op_type, version=1, source="product_stream.cu",
+            symbol=f"{symbol}_stream",
+            arguments=(arg("x", ptr, "input", index=0), *matrices, *vectors, HALF_OUT, *PRODUCT_DIMS,
+                       *((ACTIVATION,) if gated else ())) + RESERVED,
+            grid=(mul(literal(2), {"kind": "min", "args": [ceil_div(out_dim(1), literal(8)),
+                                                           ceil_div({"kind": "sm_count"}, literal(2))]}),),
+            dtype="float16", constraints=(rows_of_16_bytes, few_rows),
+            variants=(Variant("rows32", constraints=(by_rows,), **stream),
+                      Variant("rows32_turned", arg_overrides=stream_turned,
+                              constraints=(by_columns, *({"kind": "input_is_constant", "index": i} for i in weights)),
+                              **stream))))
     # One warp (rows of at most 1024 elements) or one block a row; 16 blocks
     # an SM cover the block form, whose eight resident ones hide each other's
     # barriers.

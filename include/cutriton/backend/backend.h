@@ -89,6 +89,10 @@ std::shared_ptr<Backend> CreateCudaSm100Backend();
 std::shared_ptr<Backend> CreateCudaTritonBackend();
 Status RegisterBuiltinBackends();
 
+// Whether every at_run constraint of the candidate's kernels holds for `node`
+// at the shapes of `graph`; `any` (optional) tells whether it has some.
+bool HoldsAtRun(const ExecutionCandidate& candidate, const Node& node, const Graph& graph, bool* any = nullptr);
+
 // True for target names served by the artifact-backed CUDA backend.
 bool IsCudaArtifactTarget(const std::string& target);
 // Maps a user-facing target ("cuda_triton" alias included) to a backend name.

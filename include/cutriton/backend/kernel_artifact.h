@@ -99,6 +99,11 @@ struct KernelConstraint {
   int64_t default_value{0};
   std::vector<int64_t> expected_list;
   std::vector<int64_t> default_list;
+  // kDimMultipleOf / kDimLessEqual: holds or not at the shapes of a run, not
+  // at those of the compilation (a dimension that shape profiles leave open).
+  // Lowering admits the variant either way; the context chooses it when the
+  // condition holds and never runs it when it does not.
+  bool at_run{false};
 };
 
 enum class GridExpressionKind {
