@@ -614,7 +614,7 @@ def _product_specs() -> list[KernelSpec]:
                               **pair))))
         # Few rows, weights by output channel: chosen at run time, as M is what
         # shape profiles leave open.
-        stream = dict(num_warps=8, shared_memory_bytes=229376, programmatic_launch=True)
+        stream = dict(num_warps=12, shared_memory_bytes=231424, programmatic_launch=True)
         few_rows = {"kind": "dim_le", "source": "input", "index": 0, "axis": 0, "value": 32, "at_run": 1}
         stream_turned = {a.name: {"prepack": "transpose_2d"} for a in matrices}
         specs.append(KernelSpec(
@@ -622,8 +622,7 @@ def _product_specs() -> list[KernelSpec]:
             symbol=f"{symbol}_stream",
             arguments=(arg("x", ptr, "input", index=0), *matrices, *vectors, HALF_OUT, *PRODUCT_DIMS,
                        *((ACTIVATION,) if gated else ())) + RESERVED,
-            grid=(mul(literal(2), {"kind": "min", "args": [ceil_div(out_dim(1), literal(8)),
-                                                           ceil_div({"kind": "sm_count"}, literal(2))]}),),
+            grid=({"kind": "min", "args": [ceil_div(out_dim(1), literal(8)), {"kind": "sm_count"}]},),
             dtype="float16", constraints=(rows_of_16_bytes, few_rows),
             variants=(Variant("rows32", constraints=(by_rows,), **stream),
                       Variant("rows32_turned", arg_overrides=stream_turned,
