@@ -10,13 +10,20 @@
 // bytes of k each use a block up.
 //
 // Two CTAs of a cluster (two SMs) work on one tile of 256 rows: CTA r holds
-// rows 128 r ... of x and half of the BN weight rows, and one
-// tcgen05.mma.cta_group::2 (M = 256, N = BN) reads both halves and leaves 128
-// rows of sums in each CTA's TMEM. For the gated ops the halves are the same
-// BN / 2 columns of the two weight matrices: CTA 0 loads gate rows, CTA 1 up
-// rows, and columns c and BN / 2 + c of every TMEM lane are the gate and the
-// up sum of one output, so activation and product are the epilogue of the
-// thread that reads them and neither projection ever leaves the SM.
+// rows 128 r ... of x and `half` weight rows (16 to 128), and one
+// tcgen05.mma.cta_group::2 (M = 256, N = 2 half) reads both halves and leaves
+// 128 rows of sums in each CTA's TMEM. For the gated ops the halves are the
+// same columns of the two weight matrices: CTA 0 loads gate rows, CTA 1 up
+// rows, and columns c and half + c of every TMEM lane are the gate and the up
+// sum of one output, so activation and product are the epilogue of the thread
+// that reads them and neither projection ever leaves the SM.
+//
+// The width is chosen at run time (choose_half) by what a block of K costs:
+// 4 half clocks of MMAs, 64 bytes a clock and SM through TMA (rows of x beyond
+// M are not loaded: zero-filling them took as long as loading them), or the
+// weights' share of HBM. At 512 clocks a block for half = 128 the tensor cores
+// are busy throughout (8192x4096x8192: 718 us, 1531 TFLOP/s; 8 bits
+// 8192x8192x4096: 169 us, 3253 TOP/s).
 //
 // Warp 0 loads (a ring of 192 KB), warp 1 of CTA 0 issues the MMAs into one of
 // two accumulators, 16 epilogue warps of each CTA turn the other one into
@@ -39,12 +46,11 @@ constexpr int kThreads = (2 + kEpilogueWarps) * 32;
 constexpr int kChunk = 32;
 constexpr int kEpilogueWarp0 = 2;
 constexpr int kRasterRows = 8;
-constexpr uint32_t kTileA = kBM * kRowBytes;  // 16 KB
 constexpr uint32_t kRingBytes = 196608;
 constexpr uint32_t kStageBoxBytes = 32 * kChunk * 2;
 constexpr uint32_t kStagingBytes = kEpilogueWarps * kStageBoxBytes;
-constexpr int kMaxStages = 9;
-constexpr int kSmallBox = 32;  // weight rows of the small box; the large one has 128
+constexpr int kMaxStages = 10;
+constexpr uint32_t kTmemCols = 512;  // two accumulators, 256 columns apart
 
 struct Half {
   static constexpr int kBlock = 64;  // k of a 128-byte row
@@ -59,18 +65,44 @@ struct Int8 {
   }
 };
 
-template <int BN, bool kGated>
+// Widths of a tile (weight rows a CTA) and heights of the boxes that bring
+// them and the rows of x: every block of K is one copy each, since a copy costs
+// its warp about 55 clocks whatever its size.
+constexpr int kHalves = 5;
+constexpr int kXBoxes = 3;
+__device__ __forceinline__ int half_at(int i) { return i == 0 ? 128 : i == 1 ? 96 : i == 2 ? 64 : i == 3 ? 48 : 32; }
+__device__ __forceinline__ int x_rows_at(int i) { return 128 >> i; }
+
+// A tile's width and what follows from it.
 struct Shape {
-  static constexpr int kHalf = BN / 2;                      // weight rows a CTA
-  static constexpr int kColumns = kGated ? BN / 2 : BN;     // output columns a tile
-  static constexpr uint32_t kTileB = kHalf * kRowBytes;
-  static constexpr uint32_t kStageBytes = kTileA + kTileB;  // both multiples of 1024
-  static constexpr int kStages = kRingBytes / kStageBytes;
-  static constexpr uint32_t kTmemCols = 2 * BN <= 128 ? 128 : 2 * BN <= 256 ? 256 : 512;
-  static constexpr int kChunks = kColumns / kChunk;
-  static constexpr int kActive = kChunks < kEpilogueWarps / 4 ? kChunks : kEpilogueWarps / 4;  // warps a lane quarter
-  static_assert(kStages <= kMaxStages && kHalf % kSmallBox == 0 && kColumns % kChunk == 0, "tile");
+  int width;             // index of half
+  int half;              // weight rows a CTA
+  int columns;           // output columns
+  int x_box;             // index of the box of x: the least that holds min(M, 128) rows
+  int x_bytes, block_bytes;  // of a block of K: rows of x, and with the weight rows
+  int blocks;            // of K a stage
+  int stages;
+  int chunks;            // of 32 output columns, the last one of 16 where half is 48 and gated
+  int active;            // epilogue warps a lane quarter
 };
+
+template <bool kGated>
+__device__ __forceinline__ Shape shape_of(int width, int m) {
+  Shape s;
+  s.width = width;
+  s.half = half_at(width);
+  s.columns = kGated ? s.half : 2 * s.half;
+  s.x_box = m > 64 ? 0 : m > 32 ? 1 : 2;
+  s.x_bytes = x_rows_at(s.x_box) * kRowBytes;
+  s.block_bytes = s.x_bytes + s.half * kRowBytes;  // a multiple of 1024
+  // Two blocks a stage halve the barrier rounds where a block is short; four
+  // stages at least.
+  s.blocks = s.half <= 64 ? 2 : 1;
+  s.stages = min(kMaxStages, static_cast<int>(kRingBytes) / (s.blocks * s.block_bytes));
+  s.chunks = (s.columns + kChunk - 1) / kChunk;
+  s.active = min(s.chunks, kEpilogueWarps / 4);
+  return s;
+}
 
 struct __align__(8) Barriers {
   uint64_t full[kMaxStages];   // leader: both CTAs' copies of a stage landed
@@ -80,7 +112,6 @@ struct __align__(8) Barriers {
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
-  int consumed;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -111,11 +142,28 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const TmaDescriptor*
 }
 
 // Arrives on `bar` in both CTAs when this thread's earlier MMAs are done.
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
-  const uint32_t peer = cluster_addr(bar, 1);
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-               : "memory");
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(peer) : "memory");
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
+// mbar_wait by a whole warp, which agrees on the outcome.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, void* scratch,
+                                          unsigned int site) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort, scratch, site));
+}
+
+// One lane of the warp, the same each time; the warp stays converged around it.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t elected;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(elected));
+  return elected != 0;
 }
 
 __device__ __forceinline__ void umma_pair(Half, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -170,11 +218,10 @@ __device__ __forceinline__ void tmem_load_two(uint32_t a, uint32_t b, uint32_t (
       : "memory");
 }
 
-// What the kernels bind. Weight operand o arrives through boxes of 128 or of
-// kSmallBox rows. Scales are null in FP16.
+// What the kernels bind. Scales are null in FP16.
 struct Operands {
-  const TmaDescriptor* x;
-  const TmaDescriptor* w[2][2];  // [gate / up][large box, small box]
+  const TmaDescriptor* x;     // the box of x that shape_of picks
+  const TmaDescriptor* w[2];  // [gate / up]: the box of the tile's width
   const TmaDescriptor* out_map;
   __half* out;
   const float* x_scale;
@@ -239,15 +286,12 @@ __device__ __forceinline__ void finish(const Operands& op, uint32_t (&v)[kChunk]
   }
 }
 
-template <typename T, bool kGated, int BN>
-__device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op) {
-  using S = Shape<BN, kGated>;
-  constexpr int kStages = S::kStages;
+template <typename T, bool kGated>
+__device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, const Shape sh) {
   uint8_t* staging = smem + kRingBytes;
   Barriers* bars = reinterpret_cast<Barriers*>(staging + kStagingBytes);
   volatile int* abort = &bars->abort;
-  auto tile_a = [&](int s) { return smem + s * S::kStageBytes; };
-  auto tile_b = [&](int s) { return smem + s * S::kStageBytes + kTileA; };
+  const int stage_bytes = sh.blocks * sh.block_bytes;
 
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x & 31;
@@ -256,26 +300,24 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op) 
   const int pairs = gridDim.x / 2;
   const int pair = blockIdx.x / 2;
   const int k_blocks = (op.k + T::kBlock - 1) / T::kBlock;
-  const int n_tiles = (op.n + S::kColumns - 1) / S::kColumns;
+  const int n_tiles = (op.n + sh.columns - 1) / sh.columns;
   const int m_tiles = (op.m + 2 * kBM - 1) / (2 * kBM);
   const int tiles = m_tiles * n_tiles;
   const int my_tiles = tiles > pair ? (tiles - 1 - pair) / pairs + 1 : 0;
   const bool tma_epilogue = op.n % 8 == 0 && ctb::aligned16(op.out);
-  constexpr int kBox = BN == 256 ? 0 : 1;
-  const TmaDescriptor* my_w = kGated && !leader ? op.w[1][kBox] : op.w[0][kBox];
+  const TmaDescriptor* my_w = kGated && !leader ? op.w[1] : op.w[0];
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < sh.stages; ++s) {
       mbar_init(&bars->full[s], 1);
       mbar_init(&bars->empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->tmem_full[b], 1);
-      mbar_init(&bars->tmem_empty[b], 2 * 4 * S::kActive);
+      mbar_init(&bars->tmem_empty[b], 2 * 4 * sh.active);
     }
     mbar_init(&bars->drain, 1);
     bars->abort = 0;
-    bars->consumed = 0;
     mbar_init_fence();
     tma_prefetch(op.x);
     tma_prefetch(my_w);
@@ -286,7 +328,7 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op) 
   cluster_sync();
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&bars->tmem_base)),
-                 "r"(S::kTmemCols)
+                 "r"(kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
@@ -296,83 +338,111 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op) 
   const uint32_t tmem = bars->tmem_base;
   CTB_GRID_DEPENDENCY_SYNC();
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     // ---- TMA producer: this CTA's rows of x and of the weights ----
-    int g = 0;
-    bool stop = false;
-    for (int local = 0; local < my_tiles && !stop; ++local) {
+    const uint32_t full_first = cluster_addr(&bars->full[0], 0);  // on the leader
+    int s = 0, g = 0;
+    uint32_t phase = 1;  // the first round of the ring finds every stage free
+    bool ok = true;
+    for (int local = 0; local < my_tiles && ok; ++local) {
       int mt, nt;
       tile_at(pair + local * pairs, m_tiles, n_tiles, &mt, &nt);
-      const int m0 = mt * 2 * kBM + static_cast<int>(rank) * kBM;
-      const int n0 = nt * S::kColumns + (kGated ? 0 : static_cast<int>(rank) * S::kHalf);
-      for (int kb = 0; kb < k_blocks; ++kb, ++g) {
-        const int s = g % kStages;
-        const int use = g / kStages;
-        if (use > 0 && !mbar_wait(&bars->empty[s], (use - 1) & 1, abort, op.scratch, 70)) {
-          stop = true;
+      const int pair_m0 = mt * 2 * kBM;
+      const int m0 = pair_m0 + static_cast<int>(rank) * kBM;
+      const int n0 = nt * sh.columns + (kGated ? 0 : static_cast<int>(rank) * sh.half);
+      // Rows of x past M keep what the stage held: their sums are not stored,
+      // and a CTA without rows loads none.
+      const bool has_x = m0 < op.m;
+      const int pair_bytes = 2 * sh.half * kRowBytes + (pair_m0 + kBM < op.m ? 2 : 1) * sh.x_bytes;
+      for (int kb = 0; kb < k_blocks; kb += sh.blocks) {
+        if (!warp_wait(&bars->empty[s], phase, abort, op.scratch, 70)) {
+          ok = false;
           break;
         }
-        if (leader) mbar_arrive_expect_tx(&bars->full[s], 2 * S::kStageBytes);
-        const uint32_t full_on_leader = cluster_addr(&bars->full[s], 0);
-        tma_load_2d_pair(tile_a(s), op.x, full_on_leader, kb * T::kBlock, m0);
-        if constexpr (BN == 256) {
-          tma_load_2d_pair(tile_b(s), my_w, full_on_leader, kb * T::kBlock, n0);
-        } else {
-#pragma unroll
-          for (int r = 0; r < S::kHalf; r += kSmallBox) {
-            tma_load_2d_pair(tile_b(s) + r * kRowBytes, my_w, full_on_leader, kb * T::kBlock, n0 + r);
+        if (elect_one()) {
+          const int blocks = min(sh.blocks, k_blocks - kb);
+          const uint32_t full = full_first + 8 * s;
+          if (leader) mbar_arrive_expect_tx(&bars->full[s], blocks * pair_bytes);
+          uint8_t* a = smem + s * stage_bytes;
+          for (int b = 0; b < blocks; ++b, a += sh.block_bytes) {
+            const int k0 = (kb + b) * T::kBlock;
+            if (has_x) tma_load_2d_pair(a, op.x, full, k0, m0);
+            tma_load_2d_pair(a + sh.x_bytes, my_w, full, k0, n0);
           }
+        }
+        __syncwarp();
+        ++g;
+        if (++s == sh.stages) {
+          s = 0;
+          phase ^= 1;
         }
       }
     }
-    if (*abort && leader) {
+    if (*abort && leader && lane == 0) {
       // Let the issued copies land before shared memory is released (the
       // peer's too: the leader's barrier counts them). Bounded: a phase the
       // aborted peer never fed times out after the wait limit.
-      for (int q = *reinterpret_cast<volatile int*>(&bars->consumed); q < g; ++q) {
+      for (int q = max(0, g - sh.stages); q < g; ++q) {
         volatile int never = 0;
-        mbar_wait(&bars->full[q % kStages], (q / kStages) & 1, &never, op.scratch, 71);
+        mbar_wait(&bars->full[q % sh.stages], (q / sh.stages) & 1, &never, op.scratch, 71);
       }
     }
-  } else if (warp == 1 && lane == 0 && leader) {
+    __syncwarp();
+  } else if (warp == 1 && leader) {
     // ---- MMA issuer (pair leader) ----
-    constexpr uint32_t idesc = T::idesc(2 * kBM, BN);
-    int g = 0;
+    // The whole warp runs the loop and one lane issues, so that descriptors
+    // are uniform values: by a lone thread four MMAs and two commits took 570
+    // clocks a stage, more than the 512 that the tensor cores need for it.
+    const uint32_t idesc = T::idesc(2 * kBM, 2 * sh.half);
+    const uint64_t a_first = smem_desc_kmajor_sw128(smem);
+    const uint64_t b_first = smem_desc_kmajor_sw128(smem + sh.x_bytes);
+    const uint32_t empty_first = smem_addr(&bars->empty[0]);
+    int s = 0;
+    uint32_t phase = 0;
     bool ok = true;
     for (int local = 0; local < my_tiles && ok; ++local) {
       const int buf = local & 1;
-      if (local >= 2 && !mbar_wait(&bars->tmem_empty[buf], ((local >> 1) - 1) & 1, abort, op.scratch, 72)) {
+      if (local >= 2 && !warp_wait(&bars->tmem_empty[buf], ((local >> 1) - 1) & 1, abort, op.scratch, 72)) {
         ok = false;
         break;
       }
       tc_fence_after_sync();
-      const uint32_t acc = tmem + buf * BN;
-      for (int kb = 0; kb < k_blocks; ++kb, ++g) {
-        const int s = g % kStages;
-        if (!mbar_wait(&bars->full[s], (g / kStages) & 1, abort, op.scratch, 73)) {
+      const uint32_t acc = tmem + buf * 256;
+      for (int kb = 0; kb < k_blocks; kb += sh.blocks) {
+        if (!warp_wait(&bars->full[s], phase, abort, op.scratch, 73)) {
           ok = false;
           break;
         }
         tc_fence_after_sync();
-        const uint64_t a_desc = smem_desc_kmajor_sw128(tile_a(s));
-        const uint64_t b_desc = smem_desc_kmajor_sw128(tile_b(s));
+        if (elect_one()) {
+          const int blocks = min(sh.blocks, k_blocks - kb);
+          uint32_t offset = static_cast<uint32_t>(s * stage_bytes) >> 4;
+          for (int b = 0; b < blocks; ++b, offset += static_cast<uint32_t>(sh.block_bytes) >> 4) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          umma_pair(T{}, acc, a_desc + 2 * kk, b_desc + 2 * kk, idesc, (kb | kk) != 0);
+            for (int kk = 0; kk < 4; ++kk) {
+              umma_pair(T{}, acc, a_first + offset + 2 * kk, b_first + offset + 2 * kk, idesc, (kb | b | kk) != 0);
+            }
+          }
+          umma_commit_pair(empty_first + 8 * s);
         }
-        umma_commit_pair(&bars->empty[s]);
-        *reinterpret_cast<volatile int*>(&bars->consumed) = g + 1;
+        __syncwarp();
+        if (++s == sh.stages) {
+          s = 0;
+          phase ^= 1;
+        }
       }
-      if (ok) umma_commit_pair(&bars->tmem_full[buf]);
+      if (ok && elect_one()) umma_commit_pair(smem_addr(&bars->tmem_full[buf]));
+      __syncwarp();
     }
     if (!ok) {
-      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+      if (elect_one()) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                        smem_addr(&bars->drain))
                    : "memory");
       volatile int never = 0;
       mbar_wait(&bars->drain, 0, &never, op.scratch, 74);
+      __syncwarp();
     }
-  } else if (warp >= kEpilogueWarp0 && (warp - kEpilogueWarp0) / 4 < S::kActive) {
+  } else if (warp >= kEpilogueWarp0 && (warp - kEpilogueWarp0) / 4 < sh.active) {
     // ---- epilogue: this CTA's 128 rows, quarter = warp % 4 ----
     const int quarter = warp & 3;
     const int wq = (warp - kEpilogueWarp0) / 4;
@@ -383,23 +453,23 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op) 
       int mt, nt;
       tile_at(pair + local * pairs, m_tiles, n_tiles, &mt, &nt);
       const int row0 = mt * 2 * kBM + static_cast<int>(rank) * kBM + quarter * 32;
-      const int n0 = nt * S::kColumns;
+      const int n0 = nt * sh.columns;
       const float row_scale = op.x_scale != nullptr && row0 + lane < op.m ? __ldg(op.x_scale + row0 + lane) : 0.0f;
       const bool ready = mbar_wait(&bars->tmem_full[buf], (local >> 1) & 1, abort, op.scratch, 75);
       __syncwarp();
       if (!ready) break;
       tc_fence_after_sync();
-      const uint32_t taddr = tmem + buf * BN + (static_cast<uint32_t>(quarter * 32) << 16);
+      const uint32_t taddr = tmem + buf * 256 + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
-      for (int ci = wq; ci < S::kChunks; ci += S::kActive) {
+      for (int ci = wq; ci < sh.chunks; ci += sh.active) {
         const int c = ci * kChunk;
         uint32_t v[kChunk], u[kChunk];
         if constexpr (kGated) {
-          tmem_load_two(taddr + c, taddr + S::kHalf + c, v, u);
+          tmem_load_two(taddr + c, taddr + sh.half + c, v, u);
         } else {
           tmem_load_32x32(taddr + c, v);
         }
-        if (ci + S::kActive >= S::kChunks) {
+        if (ci + sh.active >= sh.chunks) {
           // This warp's columns are in registers: release them to the issuer.
           tc_fence_before_sync();
           __syncwarp();
@@ -424,7 +494,7 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op) 
         for (int i = 0; i < kChunk / 8; ++i) {
           *reinterpret_cast<uint4*>(box_smem + lane * 64 + (((i ^ (lane >> 1)) & 3) << 4)) = packed[i];
         }
-        if (tma_epilogue) {
+        if (tma_epilogue && c + kChunk <= sh.columns) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
@@ -434,16 +504,18 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op) 
           box_used = true;
         } else {
           // Rows that TMA cannot address (N no multiple of 8, an output off
-          // 16 bytes): one row of 32 columns a store instruction.
+          // 16 bytes) and half chunks: one row of the chunk a store instruction.
           __syncwarp();
           const int column = n0 + c + lane;
+          const int end = min(op.n, n0 + sh.columns);
 #pragma unroll 4
           for (int r = 0; r < 32 && row0 + r < op.m; ++r) {
             const __half h = *reinterpret_cast<const __half*>(
                 box_smem + r * 64 + ((((lane >> 3) ^ (r >> 1)) & 3) << 4) + (lane & 7) * 2);
-            if (column < op.n) op.out[static_cast<long long>(row0 + r) * op.n + column] = h;
+            if (column < end) op.out[static_cast<long long>(row0 + r) * op.n + column] = h;
           }
           __syncwarp();
+          box_used = false;
         }
       }
     }
@@ -456,71 +528,93 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op) 
   tc_fence_after_sync();
   if (warp == 0) {
     __syncwarp();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kTmemCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
 }
 
-// Tile width: the least waves of pair tiles times a tile's cost. Both CTAs of
-// a pair compute it from the same arguments, so they agree.
+// The tile width with the least estimated clocks a block of K. A pair needs
+// 4 half clocks of MMAs for a block, and at least 250 for its round of
+// barriers and copies. From HBM the weight rows of a block come at 23 bytes a
+// clock and SM (5.6 clocks a row) when all pairs read, shared by the m_tiles
+// rows of tiles, and faster when the last wave leaves pairs idle. Every warp of
+// both CTAs gets the same answer: lane i rates width i, ties go to the widest.
+template <bool kGated>
+__device__ __forceinline__ int choose_width(int m, int n, int pairs) {
+  const int lane = threadIdx.x & 31;
+  const int half = half_at(min(lane, kHalves - 1));
+  const int columns = kGated ? half : 2 * half;
+  const int m_tiles = (m + 2 * kBM - 1) / (2 * kBM);
+  const long long tiles = static_cast<long long>(m_tiles) * ((n + columns - 1) / columns);
+  const int busy = max(4 * half, half <= 64 ? 250 : 350);
+  const int hbm = 56 * half / (10 * m_tiles);
+  const int full = static_cast<int>(min(tiles / pairs, 0x7FFFll));
+  const int rest = static_cast<int>(tiles % pairs);
+  const int clocks = full * max(busy, hbm) + (rest > 0 ? max(busy, hbm * rest / pairs) : 0);
+  const unsigned rated = static_cast<unsigned>(clocks) * 8u + static_cast<unsigned>(min(lane, kHalves - 1));
+  return static_cast<int>(__reduce_min_sync(0xFFFFFFFFu, rated) & 7u);
+}
+
+// Weight boxes of every width, by index of half.
+using Boxes = const TmaDescriptor* [kHalves];
+
 template <typename T, bool kGated>
-__device__ __forceinline__ void product_dispatch(const Operands& op) {
+__device__ __forceinline__ void product_dispatch(Operands& op, const TmaDescriptor* const (&x)[kXBoxes],
+                                                 const Boxes& w0, const Boxes& w1) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
-  const long long m_tiles = (op.m + 2 * kBM - 1) / (2 * kBM);
-  const long long pairs = gridDim.x / 2;
-  const auto cost = [&](int bn, int tile_cost) {
-    const int columns = kGated ? bn / 2 : bn;
-    const long long tiles = m_tiles * ((op.n + columns - 1) / columns);
-    return (tiles + pairs - 1) / pairs * tile_cost;
+  const Shape sh = shape_of<kGated>(choose_width<kGated>(op.m, op.n, gridDim.x / 2), op.m);
+  op.x = sh.x_box == 0 ? x[0] : sh.x_box == 1 ? x[1] : x[2];
+  const auto pick = [&](const Boxes& w) {
+    return sh.width == 0 ? w[0] : sh.width == 1 ? w[1] : sh.width == 2 ? w[2] : sh.width == 3 ? w[3] : w[4];
   };
-  const long long t256 = cost(256, 100), t192 = cost(192, 80), t128 = cost(128, 62), t64 = cost(64, 45);
-  const long long best = min(min(t256, t192), min(t128, t64));
-  if (t256 == best) {
-    product_pair<T, kGated, 256>(smem, op);
-  } else if (t192 == best) {
-    product_pair<T, kGated, 192>(smem, op);
-  } else if (t128 == best) {
-    product_pair<T, kGated, 128>(smem, op);
-  } else {
-    product_pair<T, kGated, 64>(smem, op);
-  }
+  op.w[0] = pick(w0);
+  op.w[1] = kGated ? pick(w1) : nullptr;
+  product_pair<T, kGated>(smem, op, sh);
 }
 
 }  // namespace
 
+#define CTB_X_MAPS                                                                                       \
+  const __grid_constant__ TmaDescriptor tma_x128, const __grid_constant__ TmaDescriptor tma_x64,         \
+      const __grid_constant__ TmaDescriptor tma_x32
+#define CTB_W_MAPS(name)                                                                                 \
+  const __grid_constant__ TmaDescriptor name##128, const __grid_constant__ TmaDescriptor name##96,       \
+      const __grid_constant__ TmaDescriptor name##64, const __grid_constant__ TmaDescriptor name##48,    \
+      const __grid_constant__ TmaDescriptor name##32
+
 extern "C" __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-ctb_gated_gemm_f16_pair(const __grid_constant__ TmaDescriptor tma_x, const __grid_constant__ TmaDescriptor tma_gate128,
-                        const __grid_constant__ TmaDescriptor tma_gate32,
-                        const __grid_constant__ TmaDescriptor tma_up128, const __grid_constant__ TmaDescriptor tma_up32,
+ctb_gated_gemm_f16_pair(CTB_X_MAPS, CTB_W_MAPS(tma_gate), CTB_W_MAPS(tma_up),
                         const __grid_constant__ TmaDescriptor tma_out, __half* output, int m, int n, int k,
                         int activation, CTB_RESERVED_PARAMS) {
   (void)profile_scratch;
-  const Operands op = {&tma_x,  {{&tma_gate128, &tma_gate32}, {&tma_up128, &tma_up32}},
-                       &tma_out, output, nullptr, {nullptr, nullptr}, nullptr, m, n, k, activation, runtime_scratch};
-  product_dispatch<Half, true>(op);
+  Operands op = {nullptr, {nullptr, nullptr}, &tma_out, output, nullptr, {nullptr, nullptr}, nullptr, m, n, k,
+                 activation, runtime_scratch};
+  product_dispatch<Half, true>(op, {&tma_x128, &tma_x64, &tma_x32},
+                               {&tma_gate128, &tma_gate96, &tma_gate64, &tma_gate48, &tma_gate32},
+                               {&tma_up128, &tma_up96, &tma_up64, &tma_up48, &tma_up32});
 }
 
 extern "C" __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-ctb_qgemm_i8_pair(const __grid_constant__ TmaDescriptor tma_x, const __grid_constant__ TmaDescriptor tma_w128,
-                  const __grid_constant__ TmaDescriptor tma_w32, const __grid_constant__ TmaDescriptor tma_out,
-                  const float* x_scale, const float* w_scale, const __half* bias, __half* output, int m, int n, int k,
+ctb_qgemm_i8_pair(CTB_X_MAPS, CTB_W_MAPS(tma_w), const __grid_constant__ TmaDescriptor tma_out, const float* x_scale,
+                  const float* w_scale, const __half* bias, __half* output, int m, int n, int k,
                   CTB_RESERVED_PARAMS) {
   (void)profile_scratch;
-  const Operands op = {&tma_x,  {{&tma_w128, &tma_w32}, {nullptr, nullptr}},
-                       &tma_out, output, x_scale, {w_scale, nullptr}, bias, m, n, k, 0, runtime_scratch};
-  product_dispatch<Int8, false>(op);
+  Operands op = {nullptr, {nullptr, nullptr}, &tma_out, output, x_scale, {w_scale, nullptr}, bias, m, n, k, 0,
+                 runtime_scratch};
+  product_dispatch<Int8, false>(op, {&tma_x128, &tma_x64, &tma_x32},
+                                {&tma_w128, &tma_w96, &tma_w64, &tma_w48, &tma_w32},
+                                {&tma_w128, &tma_w96, &tma_w64, &tma_w48, &tma_w32});
 }
 
 extern "C" __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-ctb_qgated_gemm_i8_pair(const __grid_constant__ TmaDescriptor tma_x, const __grid_constant__ TmaDescriptor tma_gate128,
-                        const __grid_constant__ TmaDescriptor tma_gate32,
-                        const __grid_constant__ TmaDescriptor tma_up128, const __grid_constant__ TmaDescriptor tma_up32,
+ctb_qgated_gemm_i8_pair(CTB_X_MAPS, CTB_W_MAPS(tma_gate), CTB_W_MAPS(tma_up),
                         const __grid_constant__ TmaDescriptor tma_out, const float* x_scale, const float* gate_scale,
                         const float* up_scale, __half* output, int m, int n, int k, int activation,
                         CTB_RESERVED_PARAMS) {
   (void)profile_scratch;
-  const Operands op = {&tma_x,  {{&tma_gate128, &tma_gate32}, {&tma_up128, &tma_up32}},
-                       &tma_out, output, x_scale, {gate_scale, up_scale}, nullptr, m, n, k, activation,
-                       runtime_scratch};
-  product_dispatch<Int8, true>(op);
+  Operands op = {nullptr, {nullptr, nullptr}, &tma_out, output, x_scale, {gate_scale, up_scale}, nullptr, m, n, k,
+                 activation, runtime_scratch};
+  product_dispatch<Int8, true>(op, {&tma_x128, &tma_x64, &tma_x32},
+                               {&tma_gate128, &tma_gate96, &tma_gate64, &tma_gate48, &tma_gate32},
+                               {&tma_up128, &tma_up96, &tma_up64, &tma_up48, &tma_up32});
 }

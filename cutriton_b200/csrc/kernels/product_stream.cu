@@ -1,14 +1,14 @@
-// GatedGemm, QGemm and QGatedGemm for few rows (at most 32): the weights pass
+// GatedGemm, QGemm and QGatedGemm for few rows (at most 16): the weights pass
 // once from HBM through every SM, and nothing else costs time.
 //
-// With M rows each weight takes part in M multiply-adds, so up to M = 32 the
-// product is bound by reading the weights (K N elements, twice for the gated
+// With M rows each weight takes part in M multiply-adds, so here the product is
+// bound by reading the weights (K N elements, twice for the gated
 // ops). What that needs is every SM reading at the same rate to the end and
 // enough bytes in flight (about 45 KB an SM), not tensor throughput:
 //
 // * One CTA an SM; the CTAs share the output columns out evenly in groups of
-//   8. Eight warps of a CTA take every 8th 64-byte chunk of K. A batch is four
-//   groups of weight rows (for the gated ops two of each matrix).
+//   8. The 16 reading warps of a CTA take the 64-byte chunks of K in turn. A batch is four groups of weight rows (for the gated
+//   ops two of each matrix).
 // * A warp reads a batch's chunk of 8 rows x 64 bytes with one 16-byte
 //   cp.async a lane into a queue in shared memory that is private to the
 //   lane, so the copies need no barrier: a lane waits for its own oldest
@@ -19,7 +19,7 @@
 //   {0, 1} serve as the fragment of one MMA and {2, 3} of the next. That
 //   permutes k within a chunk, and x is loaded with the same permutation
 //   through the same queue (from L2, where it stays).
-// * Four further warps join a batch's sums over the eight, in a fixed order
+// * Four further warps join a batch's sums over the readers, in a fixed order
 //   (results do not depend on timing), and store the outputs. The join buffer
 //   is double, so no reading warp waits for another one: when all of them met
 //   at a barrier after each batch (joined over a cluster of two CTAs, K split
@@ -36,7 +36,7 @@ using ctb::tc::mbar_arrive;
 using ctb::tc::mbar_init;
 using ctb::tc::mbar_wait;
 
-constexpr int kWarps = 8;      // reading warps, over which K is split
+constexpr int kWarps = 16;     // reading warps, over which K is split
 constexpr int kJoinWarps = 4;  // joining warps
 constexpr int kThreads = (kWarps + kJoinWarps) * 32;
 constexpr int kGroups = 4;   // groups of 8 weight rows a batch
@@ -83,7 +83,7 @@ struct Operands {
 };
 
 struct Barriers {
-  uint64_t full[2];   // the eight reading warps have left their sums in a join buffer
+  uint64_t full[2];   // the reading warps have left their sums in a join buffer
   uint64_t empty[2];  // the joining warps have read it
   int abort;
 };
@@ -100,7 +100,7 @@ __device__ __forceinline__ uint4 read_16(uint32_t src) {
   return v;
 }
 
-// kTokens8: groups of 8 rows of x (1, 2 or 4).
+// kTokens8: groups of 8 rows of x (1 or 2).
 template <typename T, bool kGated, int kTokens8>
 __device__ __forceinline__ void product_stream(uint8_t* smem, const Operands<T>& op) {
   using Sum = typename T::Sum;
@@ -109,7 +109,7 @@ __device__ __forceinline__ void product_stream(uint8_t* smem, const Operands<T>&
   constexpr int kTokens = 8 * kTokens8;
   constexpr int kJoin = kWarps * kTokens * kStride;  // words a join buffer
   constexpr int kDepth = (kSharedBytes - 128 - 8 * kJoin) / (kWarps * kSlotBytes);
-  static_assert(kDepth >= 4, "queue");
+  static_assert(kDepth >= 3, "queue");
   constexpr int kMTiles = (kTokens8 + 1) / 2;
   constexpr int kChannelGroups = kGated ? kGroups / 2 : kGroups;  // output groups a batch
   constexpr int kChunk = 4 * T::kPiece;
@@ -133,7 +133,7 @@ __device__ __forceinline__ void product_stream(uint8_t* smem, const Operands<T>&
   __syncthreads();
 
   if (warp < kWarps) {
-    // ---- reading warps: chunks `warp`, `warp` + 8, ... of K ----
+    // ---- reading warps: chunks `warp`, `warp` + kWarps, ... of K ----
     const int g = lane >> 2, q = lane & 3;
     const int chunks = (op.k + kChunk - 1) / kChunk;
     const int mine = chunks > warp ? (chunks - warp - 1) / kWarps + 1 : 0;
@@ -288,7 +288,7 @@ __device__ __forceinline__ void product_dispatch(const Operands<T>& op) {
   extern __shared__ __align__(16) uint8_t smem[];
   // More rows, rows of x or of weights off 16 bytes: not this kernel's (the
   // host offers it only for the rest; a tensor bound off 16 bytes ends here).
-  bool fits = op.m <= 32 && op.k % T::kPiece == 0 && ctb::aligned16(op.x) && ctb::aligned16(op.w[0]);
+  bool fits = op.m <= 16 && op.k % T::kPiece == 0 && ctb::aligned16(op.x) && ctb::aligned16(op.w[0]);
   if (kGated) fits = fits && ctb::aligned16(op.w[1]);
   if (!fits) {
     if (threadIdx.x == 0) ctb::report_error(op.scratch, ctb::kErrorBadShape, 80);
@@ -296,10 +296,8 @@ __device__ __forceinline__ void product_dispatch(const Operands<T>& op) {
   }
   if (op.m <= 8) {
     product_stream<T, kGated, 1>(smem, op);
-  } else if (op.m <= 16) {
-    product_stream<T, kGated, 2>(smem, op);
   } else {
-    product_stream<T, kGated, 4>(smem, op);
+    product_stream<T, kGated, 2>(smem, op);
   }
 }
 

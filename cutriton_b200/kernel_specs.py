@@ -587,13 +587,14 @@ def _product_specs() -> list[KernelSpec]:
         # CTA pairs: boxes are rows of 128 bytes; one variant for weights
         # given by output channel, one that turns a [K, N] constant at upload.
         block = 64 if tag == "fp16" else 128
-        maps = [arg("tma_x", "tensormap", "tensor_map", tensor="input", index=0, box=[block, 128], swizzle=128)]
+        maps = [arg(f"tma_x{rows}", "tensormap", "tensor_map", tensor="input", index=0, box=[block, rows], swizzle=128)
+                for rows in (128, 64, 32)]
         for n, i in zip(("gate", "up") if gated else ("w",), weights):
             maps += [arg(f"tma_{n}{rows}", "tensormap", "tensor_map", tensor="input", index=i, box=[block, rows],
-                         swizzle=128) for rows in (128, 32)]
+                         swizzle=128) for rows in (128, 96, 64, 48, 32)]
         maps.append(arg("tma_out", "tensormap", "tensor_map", tensor="output", index=0, box=[32, 32], swizzle=64,
                         optional=1))
-        turned = {a.name: {"prepack": "transpose_2d"} for a in maps[1:-1]}
+        turned = {a.name: {"prepack": "transpose_2d"} for a in maps[3:-1]}
         columns = 32 if gated else 64  # of the narrowest tile
         rows_of_16_bytes = {"kind": "dim_multiple_of", "source": "input", "index": 0, "axis": 1,
                             "value": 8 if tag == "fp16" else 16}
@@ -614,8 +615,8 @@ def _product_specs() -> list[KernelSpec]:
                               **pair))))
         # Few rows, weights by output channel: chosen at run time, as M is what
         # shape profiles leave open.
-        stream = dict(num_warps=12, shared_memory_bytes=231424, programmatic_launch=True)
-        few_rows = {"kind": "dim_le", "source": "input", "index": 0, "axis": 0, "value": 32, "at_run": 1}
+        stream = dict(num_warps=20, shared_memory_bytes=231424, programmatic_launch=True)
+        few_rows = {"kind": "dim_le", "source": "input", "index": 0, "axis": 0, "value": 16, "at_run": 1}
         stream_turned = {a.name: {"prepack": "transpose_2d"} for a in matrices}
         specs.append(KernelSpec(
             kernel_id=f"{name}.{tag}.stream", op_type=op_type, version=1, source="product_stream.cu",
@@ -624,8 +625,8 @@ def _product_specs() -> list[KernelSpec]:
                        *((ACTIVATION,) if gated else ())) + RESERVED,
             grid=({"kind": "min", "args": [ceil_div(out_dim(1), literal(8)), {"kind": "sm_count"}]},),
             dtype="float16", constraints=(rows_of_16_bytes, few_rows),
-            variants=(Variant("rows32", constraints=(by_rows,), **stream),
-                      Variant("rows32_turned", arg_overrides=stream_turned,
+            variants=(Variant("rows16", constraints=(by_rows,), **stream),
+                      Variant("rows16_turned", arg_overrides=stream_turned,
                               constraints=(by_columns, *({"kind": "input_is_constant", "index": i} for i in weights)),
                               **stream))))
     # One warp (rows of at most 1024 elements) or one block a row; 16 blocks
