@@ -73,6 +73,15 @@ constexpr int kXBoxes = 3;
 __device__ __forceinline__ int half_at(int i) { return i == 0 ? 128 : i == 1 ? 96 : i == 2 ? 64 : i == 3 ? 48 : 32; }
 __device__ __forceinline__ int x_rows_at(int i) { return 128 >> i; }
 
+// a / b for 0 <= a, 0 < b with 1 / b at hand: an integer division by a value
+// known at run time only takes some 150 clocks of a kernel's start.
+__device__ __forceinline__ int quotient(int a, int b, float inverse) {
+  int q = static_cast<int>(static_cast<float>(a) * inverse);
+  while (static_cast<long long>(q) * b > a) --q;
+  while (static_cast<long long>(q + 1) * b <= a) ++q;
+  return q;
+}
+
 // A tile's width and what follows from it.
 struct Shape {
   int width;             // index of half
@@ -82,12 +91,13 @@ struct Shape {
   int x_bytes, block_bytes;  // of a block of K: rows of x, and with the weight rows
   int blocks;            // of K a stage
   int stages;
+  int m_tiles, n_tiles;
   int chunks;            // of 32 output columns, the last one of 16 where half is 48 and gated
   int active;            // epilogue warps a lane quarter
 };
 
 template <bool kGated>
-__device__ __forceinline__ Shape shape_of(int width, int m) {
+__device__ __forceinline__ Shape shape_of(int width, int m, int n) {
   Shape s;
   s.width = width;
   s.half = half_at(width);
@@ -98,7 +108,9 @@ __device__ __forceinline__ Shape shape_of(int width, int m) {
   // Two blocks a stage halve the barrier rounds where a block is short; four
   // stages at least.
   s.blocks = s.half <= 64 ? 2 : 1;
-  s.stages = min(kMaxStages, static_cast<int>(kRingBytes) / (s.blocks * s.block_bytes));
+  s.stages = min(kMaxStages, static_cast<int>(kRingBytes / static_cast<float>(s.blocks * s.block_bytes)));
+  s.m_tiles = (m + 2 * kBM - 1) / (2 * kBM);
+  s.n_tiles = quotient(n + s.columns - 1, s.columns, __frcp_rn(static_cast<float>(s.columns)));
   s.chunks = (s.columns + kChunk - 1) / kChunk;
   s.active = min(s.chunks, kEpilogueWarps / 4);
   return s;
@@ -120,8 +132,11 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   return r;
 }
 
+// Without release: what the CTAs tell each other here are barrier
+// initialisations (fenced by mbar_init_fence) and that they have ended; a
+// releasing arrival waits for the epilogue's stores, 0.5 us and more.
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
@@ -233,13 +248,17 @@ struct Operands {
 
 // Tile `index` in raster order: blocks of kRasterRows tile rows, within a
 // block column by column.
-__device__ __forceinline__ void tile_at(int index, int m_tiles, int n_tiles, int* mt, int* nt) {
-  const int per_block = kRasterRows * n_tiles;
-  const int block = index / per_block;
-  const int rows = min(kRasterRows, m_tiles - block * kRasterRows);
-  const int in_block = index - block * per_block;
-  *nt = in_block / rows;
-  *mt = block * kRasterRows + in_block - *nt * rows;
+__device__ __forceinline__ void tile_at(int index, const Shape& sh, int* mt, int* nt) {
+  int first = 0;  // tile row
+  if (sh.m_tiles > kRasterRows) {
+    const int per_block = kRasterRows * sh.n_tiles;
+    const int block = quotient(index, per_block, __frcp_rn(static_cast<float>(per_block)));
+    index -= block * per_block;
+    first = block * kRasterRows;
+  }
+  const int rows = min(kRasterRows, sh.m_tiles - first);
+  *nt = rows == 1 ? index : quotient(index, rows, __frcp_rn(static_cast<float>(rows)));
+  *mt = first + index - *nt * rows;
 }
 
 // One lane's 32 outputs of a chunk: `v` the (gate) sums, `u` the up sums.
@@ -300,25 +319,18 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
   const int pairs = gridDim.x / 2;
   const int pair = blockIdx.x / 2;
   const int k_blocks = (op.k + T::kBlock - 1) / T::kBlock;
-  const int n_tiles = (op.n + sh.columns - 1) / sh.columns;
-  const int m_tiles = (op.m + 2 * kBM - 1) / (2 * kBM);
-  const int tiles = m_tiles * n_tiles;
-  const int my_tiles = tiles > pair ? (tiles - 1 - pair) / pairs + 1 : 0;
+  const int tiles = sh.m_tiles * sh.n_tiles;
   const bool tma_epilogue = op.n % 8 == 0 && ctb::aligned16(op.out);
   const TmaDescriptor* my_w = kGated && !leader ? op.w[1] : op.w[0];
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < sh.stages; ++s) {
-      mbar_init(&bars->full[s], 1);
-      mbar_init(&bars->empty[s], 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&bars->tmem_full[b], 1);
-      mbar_init(&bars->tmem_empty[b], 2 * 4 * sh.active);
-    }
-    mbar_init(&bars->drain, 1);
-    bars->abort = 0;
+  if (warp == 0) {
+    for (int i = lane; i < 2 * kMaxStages; i += 32) mbar_init(&bars->full[0] + i, 1);  // full, then empty
+    if (lane < 2) mbar_init(&bars->tmem_full[lane], 1);
+    if (lane < 2) mbar_init(&bars->tmem_empty[lane], 2 * 4 * sh.active);
+    if (lane == 2) mbar_init(&bars->drain, 1);
+    if (lane == 3) bars->abort = 0;
     mbar_init_fence();
+  } else if (warp == 1 && lane == 0) {
     tma_prefetch(op.x);
     tma_prefetch(my_w);
     if (tma_epilogue) tma_prefetch(op.out_map);
@@ -344,9 +356,9 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
     int s = 0, g = 0;
     uint32_t phase = 1;  // the first round of the ring finds every stage free
     bool ok = true;
-    for (int local = 0; local < my_tiles && ok; ++local) {
+    for (int tile = pair; tile < tiles && ok; tile += pairs) {
       int mt, nt;
-      tile_at(pair + local * pairs, m_tiles, n_tiles, &mt, &nt);
+      tile_at(tile, sh, &mt, &nt);
       const int pair_m0 = mt * 2 * kBM;
       const int m0 = pair_m0 + static_cast<int>(rank) * kBM;
       const int n0 = nt * sh.columns + (kGated ? 0 : static_cast<int>(rank) * sh.half);
@@ -400,7 +412,7 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
     int s = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int local = 0; local < my_tiles && ok; ++local) {
+    for (int tile = pair, local = 0; tile < tiles && ok; tile += pairs, ++local) {
       const int buf = local & 1;
       if (local >= 2 && !warp_wait(&bars->tmem_empty[buf], ((local >> 1) - 1) & 1, abort, op.scratch, 72)) {
         ok = false;
@@ -448,10 +460,10 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
     const int wq = (warp - kEpilogueWarp0) / 4;
     uint8_t* box_smem = staging + (warp - kEpilogueWarp0) * kStageBoxBytes;
     bool box_used = false;
-    for (int local = 0; local < my_tiles; ++local) {
+    for (int tile = pair, local = 0; tile < tiles; tile += pairs, ++local) {
       const int buf = local & 1;
       int mt, nt;
-      tile_at(pair + local * pairs, m_tiles, n_tiles, &mt, &nt);
+      tile_at(tile, sh, &mt, &nt);
       const int row0 = mt * 2 * kBM + static_cast<int>(rank) * kBM + quarter * 32;
       const int n0 = nt * sh.columns;
       const float row_scale = op.x_scale != nullptr && row0 + lane < op.m ? __ldg(op.x_scale + row0 + lane) : 0.0f;
@@ -519,7 +531,8 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
         }
       }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    // The boxes have been read (the stores end with the kernel).
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -532,25 +545,34 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
   }
 }
 
-// The tile width with the least estimated clocks a block of K. A pair needs
-// 4 half clocks of MMAs for a block, and at least 250 for its round of
-// barriers and copies. From HBM the weight rows of a block come at 23 bytes a
-// clock and SM (5.6 clocks a row) when all pairs read, shared by the m_tiles
-// rows of tiles, and faster when the last wave leaves pairs idle. Every warp of
-// both CTAs gets the same answer: lane i rates width i, ties go to the widest.
+// The tile width with the least estimated clocks a block of K. A pair takes
+// 4 half clocks of MMAs for a block plus 52, and no less than its round of
+// barriers and copies (measured 295 clocks with 32 rows of x, 375 with 128).
+// From HBM the weight rows of a block come at 23 bytes a clock and SM (5.6
+// clocks a row) when all pairs read, shared by the m_tiles rows of tiles, and
+// faster when the last wave leaves pairs idle. So few rows take the width that
+// keeps HBM busy in the last wave too (32x4096x12288: half 96 or 64 44 us, 128
+// 51 us, 32 60 us), many rows the widest (512x4096x11008 in 8 bits: 128 39 us,
+// 64 42 us, 32 62 us), and a single wave the narrowest (100x12288x1504: 32 37
+// us, 128 61 us). Every warp of both CTAs gets the same answer: lane i rates
+// width i, ties go to the widest.
 template <bool kGated>
 __device__ __forceinline__ int choose_width(int m, int n, int pairs) {
   const int lane = threadIdx.x & 31;
-  const int half = half_at(min(lane, kHalves - 1));
-  const int columns = kGated ? half : 2 * half;
-  const int m_tiles = (m + 2 * kBM - 1) / (2 * kBM);
-  const long long tiles = static_cast<long long>(m_tiles) * ((n + columns - 1) / columns);
-  const int busy = max(4 * half, half <= 64 ? 250 : 350);
-  const int hbm = 56 * half / (10 * m_tiles);
-  const int full = static_cast<int>(min(tiles / pairs, 0x7FFFll));
-  const int rest = static_cast<int>(tiles % pairs);
-  const int clocks = full * max(busy, hbm) + (rest > 0 ? max(busy, hbm * rest / pairs) : 0);
-  const unsigned rated = static_cast<unsigned>(clocks) * 8u + static_cast<unsigned>(min(lane, kHalves - 1));
+  const int width = min(lane, kHalves - 1);
+  const float half = static_cast<float>(half_at(width));
+  const float columns = kGated ? half : 2.0f * half;
+  const float m_tiles = static_cast<float>((m + 2 * kBM - 1) / (2 * kBM));
+  const float tiles = m_tiles * ceilf(__fdividef(static_cast<float>(n), columns));
+  const float x_rows = m > 64 ? 128.0f : m > 32 ? 64.0f : 32.0f;
+  const float busy = fmaxf(4.0f * half + 52.0f, 268.0f + 0.85f * x_rows);
+  const float hbm = __fdividef(5.6f * half, m_tiles);
+  const float waves = __fdividef(tiles, static_cast<float>(pairs));
+  const float full = floorf(waves + 1e-3f);
+  const float rest = fmaxf(0.0f, waves - full);
+  float clocks = full * fmaxf(busy, hbm) + (rest > 1e-3f ? fmaxf(busy, hbm * rest) : 0.0f);
+  if (full == 0.0f) clocks += half / 16.0f;
+  const unsigned rated = static_cast<unsigned>(fminf(clocks, 2e8f)) * 8u + static_cast<unsigned>(width);
   return static_cast<int>(__reduce_min_sync(0xFFFFFFFFu, rated) & 7u);
 }
 
@@ -562,7 +584,7 @@ __device__ __forceinline__ void product_dispatch(Operands& op, const TmaDescript
                                                  const Boxes& w0, const Boxes& w1) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
-  const Shape sh = shape_of<kGated>(choose_width<kGated>(op.m, op.n, gridDim.x / 2), op.m);
+  const Shape sh = shape_of<kGated>(choose_width<kGated>(op.m, op.n, gridDim.x / 2), op.m, op.n);
   op.x = sh.x_box == 0 ? x[0] : sh.x_box == 1 ? x[1] : x[2];
   const auto pick = [&](const Boxes& w) {
     return sh.width == 0 ? w[0] : sh.width == 1 ? w[1] : sh.width == 2 ? w[2] : sh.width == 3 ? w[3] : w[4];
