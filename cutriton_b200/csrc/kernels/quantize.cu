@@ -6,166 +6,287 @@
 // an integer. A row of zeros has s = 0 and q = 0. A row that holds an infinity
 // or a NaN has s = inf or NaN and q = 0, so that a product with it is NaN.
 //
-// One pass over HBM (3 bytes an element): a row is read into registers, its
-// maximum found, and the integers written from the registers; only rows above
-// kCached vectors a thread read their tail again (from L2). Element i of x
-// and of q have the same flat index, so a vector of 8 elements that starts at
-// a multiple of 8 is 16-byte aligned in x and 8-byte aligned in q whatever
-// the row length: rows of odd length move by whole vectors too, and the one
-// or two vectors that a row shares with its neighbours element by element.
-// Rows of at most 1024 elements take a warp each (eight a block), longer
-// ones a block: a block's two barriers cost more than a short row's transfer.
+// One pass over HBM (3 bytes an element). A warp (two or four for long rows)
+// takes whole rows and waits for no other one: each lane copies its vectors of
+// 8 elements into a queue of its own in shared memory (cp.async), 13.5 KB a warp,
+// finds the row's maximum, and reads them back to write the integers. So 216 KB
+// of an SM's rows are under way while sixteen warps compute, which needs 10 of
+// the 16 lane instructions an element that full HBM rate leaves. (With rows in
+// registers, by blocks of 256 threads with two barriers a row, 16384x8192 ran
+// at 4.2 TB/s and 16384x2048 at 1.9; unrolled over 16 vectors a lane the code
+// outgrew the instruction cache, 1.8.)
+//
+// Element i of x and of q have the same flat index, so a vector of 8 elements
+// that starts at a multiple of 8 is 16-byte aligned in x and 8-byte aligned in
+// q whatever the row length: rows of odd length move by whole vectors too, all
+// but the one or two that a row shares with its neighbours.
 
 #include "common.cuh"
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int kCached = 4;             // vectors of 8 elements a thread holds: 8192 elements a block
-constexpr int kWarpRow = 1024;         // longest row of the warp form (4 vectors a lane)
+constexpr int kWarps = 16;
+constexpr int kThreads = kWarps * 32;
+constexpr int kSlots = 27;  // vectors of 8 elements that a lane's queue holds
+static_assert(kWarps <= 16, "row_maximum numbers its barriers by warps, from 1; there are 16");
 constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer, half to even
 
-// Eight consecutive elements as bits; those outside [begin, end) read as 0.
-__device__ __forceinline__ uint4 load_vector(const unsigned short* __restrict__ x, long long at, long long begin,
-                                             long long end, bool aligned) {
-  if (aligned && at >= begin && at + 8 <= end) return __ldg(reinterpret_cast<const uint4*>(x + at));
-  uint32_t w[4] = {0, 0, 0, 0};
+// Largest |x| of each FP16 half, NaN if one is.
+__device__ __forceinline__ __half2 largest(uint4 v, __half2 m) {
+  const __half2* h = reinterpret_cast<const __half2*>(&v);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t bits = at + e >= begin && at + e < end ? x[at + e] : 0u;
-    w[e / 2] |= bits << (16 * (e & 1));
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// Largest |x| of each 16-bit half as its bits: magnitudes order like
-// integers, infinity above every number and NaN above infinity.
-__device__ __forceinline__ uint32_t largest(uint4 v, uint32_t m) {
-  m = __vmaxu2(m, v.x & 0x7FFF7FFFu);
-  m = __vmaxu2(m, v.y & 0x7FFF7FFFu);
-  m = __vmaxu2(m, v.z & 0x7FFF7FFFu);
-  return __vmaxu2(m, v.w & 0x7FFF7FFFu);
+  for (int e = 0; e < 4; ++e) m = __hmax2_nan(m, __habs2(h[e]));
+  return m;
 }
 
 // round_half_even(x / s) from the approximate quotient's rounding q, off by
 // at most one. r = x - q s is exact: x and s are multiples of s's last place
 // (|x| >= s / 2 here and x has 11 bits to s's 24) and |r| < s.
-__device__ __noinline__ float settle(float x, float s, float q) {
+__device__ __forceinline__ float settle(float x, float s, float q) {
   const float r = fmaf(-q, s, x);
   const float twice = 2.0f * fabsf(r);
-  const bool odd = fmodf(q, 2.0f) != 0.0f;
+  const bool odd = (static_cast<int>(q) & 1) != 0;
   return twice > s || (twice == s && odd) ? q + copysignf(1.0f, r) : q;
 }
 
-// Eight integers of one vector, a byte each.
-__device__ __forceinline__ uint2 quantize(uint4 v, float s, float inv) {
+// The low byte of kMagic + n is the integer n in two's complement.
+__device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
+  return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040),
+                     __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
+}
+
+__device__ __noinline__ uint2 quantize_settled(uint4 v, float s, float inv) {
   const __half2* h = reinterpret_cast<const __half2*>(&v);
-  float x[8], t[8];
-  float border = 0.0f;
+  float t[8];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float2 f = __half22float2(h[e]);
-    x[2 * e] = f.x;
-    x[2 * e + 1] = f.y;
+    t[2 * e] = kMagic + settle(f.x, s, fmaf(f.x, inv, kMagic) - kMagic);
+    t[2 * e + 1] = kMagic + settle(f.y, s, fmaf(f.y, inv, kMagic) - kMagic);
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    t[e] = fmaf(x[e], inv, kMagic);
-    border = fmaxf(border, fabsf(fmaf(x[e], inv, kMagic - t[e])));
-  }
-  // inv is off by 2^-24 relative and |x inv| <= 127, so a quotient whose
-  // distance to its integer is below 0.5 - 2^-15 is rounded rightly.
-  if (border > 0.49996f) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) t[e] = kMagic + settle(x[e], s, t[e] - kMagic);
-  }
-  // The low byte of t's bits is the integer in two's complement.
-  uint32_t w[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t lo = __byte_perm(__float_as_uint(t[4 * i]), __float_as_uint(t[4 * i + 1]), 0x0040);
-    const uint32_t hi = __byte_perm(__float_as_uint(t[4 * i + 2]), __float_as_uint(t[4 * i + 3]), 0x0040);
-    w[i] = __byte_perm(lo, hi, 0x5410);
-  }
-  return make_uint2(w[0], w[1]);
+  return make_uint2(low_bytes(t[0], t[1], t[2], t[3]), low_bytes(t[4], t[5], t[6], t[7]));
 }
 
-__device__ __forceinline__ void store_vector(signed char* __restrict__ q, long long at, long long begin, long long end,
-                                             bool aligned, uint2 w) {
-  if (aligned && at >= begin && at + 8 <= end) {
-    *reinterpret_cast<uint2*>(q + at) = w;
-    return;
+// Eight integers of one vector, a byte each. inv is 1 / s to 2^-22: |x inv|
+// is at most 127.1, so a quotient is off by less than 2^-15 + 2^-17 and where
+// its roundings with an inverse 2^-21 smaller and larger agree (the tests'
+// 2^-21 of 127 is 2^-14), the exact one does too. Else it is settled exactly.
+__device__ __forceinline__ uint2 quantize(uint4 v, float s, float inv) {
+  const __half2* h = reinterpret_cast<const __half2*>(&v);
+  const float below = inv * (1.0f - 0x1p-21f), above = inv * (1.0f + 0x1p-21f);
+  float t[8], u[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 f = __half22float2(h[e]);
+    t[2 * e] = fmaf(f.x, below, kMagic);
+    t[2 * e + 1] = fmaf(f.y, below, kMagic);
+    u[2 * e] = fmaf(f.x, above, kMagic);
+    u[2 * e + 1] = fmaf(f.y, above, kMagic);
   }
+  const uint2 a = make_uint2(low_bytes(t[0], t[1], t[2], t[3]), low_bytes(t[4], t[5], t[6], t[7]));
+  const uint2 b = make_uint2(low_bytes(u[0], u[1], u[2], u[3]), low_bytes(u[4], u[5], u[6], u[7]));
+  return ((a.x ^ b.x) | (a.y ^ b.y)) == 0 ? a : quantize_settled(v, s, inv);
+}
+
+// A row as vectors of 8 elements from the multiple of 8 at or before its
+// first one; `head` elements of the first vector and those of the last one
+// from `tail` on are not the row's.
+struct Row {
+  const uint4* x;
+  uint2* q;
+  int vectors, head, tail;
+};
+
+// Vector i without the elements that are not the row's.
+__device__ __forceinline__ uint4 trimmed(const Row& r, int i, uint4 v) {
+  const int lo = i == 0 ? r.head : 0, hi = i == r.vectors - 1 ? r.tail : 8;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    if (at + e >= begin && at + e < end) q[at + e] = static_cast<signed char>((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
+    if (e < lo || e >= hi) w[e / 2] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+  }
+  return v;
+}
+
+// The row's elements of vector i, written one by one.
+__device__ __forceinline__ void store_elements(const Row& r, int i, uint2 w) {
+  const int lo = i == 0 ? r.head : 0, hi = i == r.vectors - 1 ? r.tail : 8;
+  signed char* q = reinterpret_cast<signed char*>(r.q + i);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (e >= lo && e < hi) q[e] = static_cast<signed char>((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
   }
 }
 
-// One row by `kLanes` threads (a warp or the block), `lane` of them this one.
-template <int kLanes>
-__device__ __forceinline__ void quantize_row(const unsigned short* __restrict__ x, signed char* __restrict__ q,
-                                             float* __restrict__ scale, long long row, int columns, int lane,
-                                             bool aligned, uint32_t* shared) {
-  const long long begin = row * columns, end = begin + columns;
-  const long long first = begin & ~7ll;
-  const int vectors = static_cast<int>((end - first + 7) >> 3);
-  uint4 v[kCached];
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < kCached; ++j) {
-    const int i = j * kLanes + lane;
-    v[j] = i < vectors ? load_vector(x, first + 8ll * i, begin, end, aligned) : make_uint4(0, 0, 0, 0);
-  }
-#pragma unroll
-  for (int j = 0; j < kCached; ++j) m = largest(v[j], m);
-  for (int i = kCached * kLanes + lane; i < vectors; i += kLanes) {
-    m = largest(load_vector(x, first + 8ll * i, begin, end, aligned), m);
-  }
-  m = max(m & 0xFFFFu, m >> 16);
+// Copies one vector to shared memory: its first `bytes` bytes, zeros for the rest.
+__device__ __forceinline__ void copy_vector(uint32_t dst, const uint4* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ uint4 read_vector(uint32_t src) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src)
+               : "memory");
+  return v;
+}
+
+// The maximum of a row over its `warps` warps (a power of two).
+__device__ __forceinline__ uint32_t row_maximum(uint32_t m, int warps, uint32_t* shared) {
   m = __reduce_max_sync(0xFFFFFFFFu, m);
-  if (kLanes > 32) {
-    __syncthreads();  // the previous row's readers are done with `shared`
-    if ((threadIdx.x & 31) == 0) shared[threadIdx.x / 32] = m;
-    __syncthreads();
-    m = __reduce_max_sync(0xFFFFFFFFu, shared[threadIdx.x & (kWarps - 1)]);
+  if (warps > 1) {
+    const int warp = threadIdx.x / 32, first = warp & ~(warps - 1), barrier = 1 + first;
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(32 * warps) : "memory");  // the last row's readers are done
+    if ((threadIdx.x & 31) == 0) shared[warp] = m;
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(32 * warps) : "memory");
+    for (int w = 0; w < warps; ++w) m = max(m, shared[first + w]);
   }
-  const float amax = __half2float(__ushort_as_half(static_cast<unsigned short>(m)));
-  const float s = __fdiv_rn(amax, 127.0f);
-  if (lane == 0) scale[row] = s;
-  const bool regular = m != 0 && m < 0x7C00u;
-  const float inv = regular ? __fdiv_rn(1.0f, s) : 0.0f;
-#pragma unroll
-  for (int j = 0; j < kCached; ++j) {
-    const int i = j * kLanes + lane;
-    if (i < vectors) {
-      store_vector(q, first + 8ll * i, begin, end, aligned, regular ? quantize(v[j], s, inv) : make_uint2(0, 0));
+  return m;
+}
+
+// fl32(amax / 127) for FP16 amax: the product with fl32(1 / 127) corrected by
+// its exact remainder, which rounds as the division does (P. Markstein, 1990).
+__device__ __forceinline__ float scale_of(float amax) {
+  const float inverse = 1.0f / 127.0f;
+  const float s = amax * inverse;
+  return amax < INFINITY ? fmaf(fmaf(-s, 127.0f, amax), inverse, s) : amax;
+}
+
+__device__ __forceinline__ Row row_at(const unsigned short* x, signed char* q, long long row, int columns) {
+  const long long begin = row * columns, first = begin & ~7ll;
+  Row r;
+  r.x = reinterpret_cast<const uint4*>(x + first);
+  r.q = reinterpret_cast<uint2*>(q + first);
+  r.head = static_cast<int>(begin - first);
+  r.vectors = (r.head + columns + 7) >> 3;
+  r.tail = r.head + columns - 8 * (r.vectors - 1);
+  return r;
+}
+
+// Batches of `batch` rows of `slots` vectors a lane, kAhead batches in the
+// queue, by groups of `warps` warps.
+template <int kAhead>
+__device__ __forceinline__ void quantize_rows(uint8_t* smem, const unsigned short* __restrict__ x,
+                                              signed char* __restrict__ q, float* __restrict__ scale, int rows,
+                                              int columns, int warps_log2, int slots, int batch,
+                                              uint32_t* shared) {
+  const int warps = 1 << warps_log2, lanes_log2 = 5 + warps_log2, lanes = 1 << lanes_log2;
+  const int group_in_block = threadIdx.x >> lanes_log2;
+  const int lane = threadIdx.x & (lanes - 1);
+  const int groups_a_block = kWarps >> warps_log2;
+  const long long groups = static_cast<long long>(gridDim.x) * groups_a_block;
+  const long long group = static_cast<long long>(blockIdx.x) * groups_a_block + group_in_block;
+  const long long total = static_cast<long long>(rows) * columns;
+  const uint32_t queue = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + (threadIdx.x / 32) * (kSlots * 512) +
+                         (threadIdx.x & 31) * 16;
+  const uint32_t batch_bytes = static_cast<uint32_t>(batch * slots) * 512;
+
+  long long fetch = group * batch;  // first row of the next batch to copy
+  int place = 0;                    // of the next batch in the queue
+  const auto copy_batch = [&]() {
+    for (int k = 0; k < batch && fetch + k < rows; ++k) {
+      const Row r = row_at(x, q, fetch + k, columns);
+      // The tensor's last vector may end past it.
+      const long long end = (fetch + k) * columns - r.head + 8ll * r.vectors;
+      const int last_bytes = end > total ? 16 - 2 * static_cast<int>(end - total) : 16;
+      const uint32_t dst = queue + place * batch_bytes + static_cast<uint32_t>(k * slots) * 512;
+      const int mine = lane < r.vectors ? ((r.vectors - lane - 1) >> lanes_log2) + 1 : 0;
+#pragma unroll 4
+      for (int j = 0; j < mine; ++j) {
+        const int i = (j << lanes_log2) + lane;
+        copy_vector(dst + j * 512, r.x + i, i == r.vectors - 1 ? last_bytes : 16);
+      }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    fetch += groups * batch;
+    place = place + 1 == kAhead ? 0 : place + 1;
+  };
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a) copy_batch();
+
+  int at = 0;
+  for (long long row0 = group * batch; row0 < rows; row0 += groups * batch) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+    for (int k = 0; k < batch && row0 + k < rows; ++k) {
+      const Row r = row_at(x, q, row0 + k, columns);
+      const bool ragged = r.head != 0 || r.tail != 8;
+      const uint32_t src = queue + at * batch_bytes + static_cast<uint32_t>(k * slots) * 512;
+      __half2 pair = __half2half2(__ushort_as_half(0));
+      const int mine = lane < r.vectors ? ((r.vectors - lane - 1) >> lanes_log2) + 1 : 0;
+#pragma unroll 4
+      for (int j = 0; j < mine; ++j) {
+        const int i = (j << lanes_log2) + lane;
+        uint4 v = read_vector(src + j * 512);
+        if (ragged && (i == 0 || i == r.vectors - 1)) v = trimmed(r, i, v);
+        pair = largest(v, pair);
+      }
+      const uint32_t bits = *reinterpret_cast<uint32_t*>(&pair) & 0x7FFF7FFFu;
+      const uint32_t m = row_maximum(max(bits & 0xFFFFu, bits >> 16), warps, shared);
+      const float s = scale_of(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+      if (lane == 0) scale[row0 + k] = s;
+      float inv;
+      asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(s));
+      const bool regular = m != 0 && m < 0x7C00u;
+#pragma unroll 4
+      for (int j = 0; j < mine; ++j) {
+        const int i = (j << lanes_log2) + lane;
+        const uint2 packed = regular ? quantize(read_vector(src + j * 512), s, inv) : make_uint2(0, 0);
+        if (ragged && (i == 0 || i == r.vectors - 1)) {
+          store_elements(r, i, packed);
+        } else {
+          r.q[i] = packed;
+        }
+      }
+    }
+    at = at + 1 == kAhead ? 0 : at + 1;
+    // The batch's last values are in registers: its place may be overwritten.
+    copy_batch();
   }
-  for (int i = kCached * kLanes + lane; i < vectors; i += kLanes) {
-    const uint4 again = load_vector(x, first + 8ll * i, begin, end, aligned);
-    store_vector(q, first + 8ll * i, begin, end, aligned, regular ? quantize(again, s, inv) : make_uint2(0, 0));
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// One row by a block, element by element: tensors off 16 bytes (x) or 8 (q), and
+// rows longer than the queues of four warps.
+__device__ __forceinline__ void quantize_row_unaligned(const unsigned short* __restrict__ x,
+                                                       signed char* __restrict__ q, float* __restrict__ scale,
+                                                       long long row, int columns, uint32_t* shared) {
+  const unsigned short* xr = x + row * columns;
+  uint32_t m = 0;
+  for (int i = threadIdx.x; i < columns; i += kThreads) m = max(m, static_cast<uint32_t>(xr[i]) & 0x7FFFu);
+  m = row_maximum(m, kWarps, shared);
+  const float s = scale_of(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+  if (threadIdx.x == 0) scale[row] = s;
+  const bool regular = m != 0 && m < 0x7C00u;
+  const float inv = regular ? __frcp_rn(s) : 0.0f;
+  for (int i = threadIdx.x; i < columns; i += kThreads) {
+    const float f = __half2float(__ushort_as_half(xr[i]));
+    q[row * columns + i] = regular ? static_cast<signed char>(settle(f, s, rintf(f * inv))) : 0;
   }
 }
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(kThreads)
+extern "C" __global__ void __launch_bounds__(kThreads, 1)
 ctb_quantize_rows_f16(const unsigned short* x, signed char* q, float* scale, int rows, int columns,
                       CTB_RESERVED_PARAMS) {
   CTB_UNUSED_RESERVED();
   CTB_GRID_DEPENDENCY_SYNC();
-  __shared__ uint32_t shared[kWarps];
-  const bool aligned = ctb::aligned16(x) && (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
-  if (columns <= kWarpRow) {
-    const int stride = gridDim.x * kWarps;
-    for (int row = blockIdx.x * kWarps + threadIdx.x / 32; row < rows; row += stride) {
-      quantize_row<32>(x, q, scale, row, columns, threadIdx.x & 31, aligned, shared);
-    }
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint32_t* shared = reinterpret_cast<uint32_t*>(smem + kWarps * kSlots * 512);
+  const int vectors = columns / 8 + 2;  // at most: a row may begin and end inside a vector
+  if (!ctb::aligned16(x) || (reinterpret_cast<uintptr_t>(q) & 7u) != 0 || vectors > 4 * 32 * kSlots) {
+    for (int row = blockIdx.x; row < rows; row += gridDim.x) quantize_row_unaligned(x, q, scale, row, columns, shared);
     return;
   }
-  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
-    quantize_row<kThreads>(x, q, scale, row, columns, threadIdx.x, aligned, shared);
+  // One warp where two rows fit its queue; four where rows are few (latency
+  // counts, not rate).
+  const bool few = rows <= static_cast<int>(gridDim.x) * (kWarps / 4) && vectors > 64;
+  const int warps_log2 = few || vectors > 64 * (kSlots / 2) ? 2 : vectors > 32 * (kSlots / 2) ? 1 : 0;
+  const int slots = (vectors + (32 << warps_log2) - 1) >> (5 + warps_log2);
+  if (slots > kSlots / 2) {
+    quantize_rows<1>(smem, x, q, scale, rows, columns, warps_log2, slots, 1, shared);
+  } else if (slots > kSlots / 4) {
+    quantize_rows<2>(smem, x, q, scale, rows, columns, warps_log2, slots, 1, shared);
+  } else {
+    quantize_rows<4>(smem, x, q, scale, rows, columns, warps_log2, slots, kSlots / 4 / slots, shared);
   }
 }

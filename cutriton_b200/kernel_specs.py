@@ -629,18 +629,15 @@ def _product_specs() -> list[KernelSpec]:
                       Variant("rows16_turned", arg_overrides=stream_turned,
                               constraints=(by_columns, *({"kind": "input_is_constant", "index": i} for i in weights)),
                               **stream))))
-    # One warp (rows of at most 1024 elements) or one block a row; 16 blocks
-    # an SM cover the block form, whose eight resident ones hide each other's
-    # barriers.
+    # One block of sixteen warps an SM: a queue of 13.5 KB a warp, and its maxima.
     specs.append(KernelSpec(
         kernel_id="quantize_rows.fp16", op_type="QuantizeRows", version=1, source="quantize.cu",
         symbol="ctb_quantize_rows_f16", dtype="int8",
         arguments=(arg("x", "*fp16", "input", index=0), arg("q", "*i8", "output", index=0),
                    arg("scale", "*fp32", "output", index=1), arg("rows", "i32", "input_dim", index=0, axis=0),
                    arg("columns", "i32", "input_dim", index=0, axis=1)) + RESERVED,
-        grid=({"kind": "min", "args": [{"kind": "input_dim", "index": 0, "axis": 0},
-                                       mul({"kind": "sm_count"}, literal(16))]},),
-        variants=(Variant("row_in_registers", num_warps=8, default=True, programmatic_launch=True),)))
+        grid=({"kind": "min", "args": [{"kind": "input_dim", "index": 0, "axis": 0}, {"kind": "sm_count"}]},),
+        variants=(Variant("row_queues", num_warps=16, shared_memory_bytes=16 * 27 * 512 + 64, default=True, programmatic_launch=True),)))
     return specs
 
 
