@@ -18,8 +18,10 @@ has no kernels (and the reference's returns Unsupported too).
 ONNX operators map onto the engine's op set: Conv (group 1, no bias), BatchNormalization, Relu, Add,
 MaxPool, GlobalAveragePool, Flatten (axis 1), Gemm / MatMul (2-D, no bias;
 a constant B with transB = 1 is transposed at import), Gelu, LayerNormalization
-(last axis), Softmax (last axis), SkipLayerNormalization. Anything else raises
-:class:`UnsupportedModelError` naming the node.
+(last axis), Softmax (last axis), SkipLayerNormalization, Mul and Silu. The
+engine's own GatedGemm, QuantizeRows, QGemm and QGatedGemm are taken by name
+(``activation``: "silu" or "gelu"; ``transB`` as it is; int8 constants).
+Anything else raises :class:`UnsupportedModelError` naming the node.
 """
 
 from __future__ import annotations
@@ -31,7 +33,7 @@ from typing import Any, Mapping
 
 import numpy as np
 
-from . import FLOAT16, Model, build_engine
+from . import FLOAT16, FLOAT32, INT8, Model, build_engine
 from .onnx_import import load_onnx
 
 SUPPORTED_TARGETS = {"cuda_sm100", "cuda_triton", "cpu_reference"}
@@ -82,8 +84,11 @@ def _normalise_json(doc: dict[str, Any], default_name: str) -> dict[str, Any]:
             "input_dtypes": dict(doc.get("input_dtypes") or {}), "nodes": nodes, "constants": constants}
 
 
-_SIMPLE = {"Relu", "Add", "GlobalAveragePool", "Gelu", "SkipLayerNormalization"}
-_KNOWN = _SIMPLE | {"Conv", "BatchNormalization", "MaxPool", "Flatten", "Gemm", "MatMul", "LayerNormalization",
+_SIMPLE = {"Relu", "Add", "Mul", "Silu", "GlobalAveragePool", "Gelu", "SkipLayerNormalization", "QuantizeRows"}
+_PRODUCTS = {"GatedGemm", "QGemm", "QGatedGemm"}
+_ACTIVATIONS = {"silu": 0, "gelu": 1}
+_OUTPUT_DTYPES = {FLOAT16: np.float16, FLOAT32: np.float32, INT8: np.int8}
+_KNOWN = _SIMPLE | _PRODUCTS | {"Conv", "BatchNormalization", "MaxPool", "Flatten", "Gemm", "MatMul", "LayerNormalization",
                     "Softmax"}
 
 
@@ -148,6 +153,13 @@ def _to_model(ir: dict[str, Any], shapes: dict[str, tuple[int, ...]], dtypes: di
             if attrs.get("approximate", "none") not in ("none", ""):
                 raise UnsupportedModelError(f"{where}: only the exact (erf) GELU is supported")
             out = {}
+        elif op in _PRODUCTS:
+            out = {"transB": int(attrs.get("transB", 0))}
+            if op != "QGemm":
+                activation = attrs.get("activation", "silu")
+                if activation not in _ACTIVATIONS and activation not in _ACTIVATIONS.values():
+                    raise UnsupportedModelError(f"{where}: activation must be 'silu' or 'gelu'")
+                out["activation"] = _ACTIVATIONS.get(activation, activation)
         else:
             out = {}
         used.update(ins)
@@ -158,7 +170,7 @@ def _to_model(ir: dict[str, Any], shapes: dict[str, tuple[int, ...]], dtypes: di
         array = np.asarray(array)
         if array.dtype == np.float64:
             array = array.astype(np.float32)
-        if array.dtype not in (np.float32, np.float16):
+        if array.dtype not in (np.float32, np.float16, np.int8):
             raise UnsupportedModelError(f"constant {name!r}: dtype {array.dtype} is not supported")
         model.add_constant(name, array, layout="OIHW" if name in conv_weights else "")
     for name, op, ins, outs, attrs in nodes:
@@ -224,13 +236,12 @@ class ExecutionContext:
                 ctx.bind_tensor(n, device[n])
             for n in plan["outputs"]:
                 code, shape = native.value_desc(n)
-                dtype = np.float16 if code == FLOAT16 else np.float32
-                device[n] = torch.empty(shape, dtype=getattr(torch, np.dtype(dtype).name), device="cuda")
+                device[n] = torch.empty(shape, dtype=getattr(torch, np.dtype(_OUTPUT_DTYPES[code]).name), device="cuda")
                 ctx.bind_tensor(n, device[n], output=True)
             entry = (ctx, device)
             self._contexts[id(native)] = entry
         ctx, device = entry
-        outputs = {n: np.empty(tuple(device[n].shape), dtype=np.float16 if device[n].dtype == torch.float16
-                               else np.float32) for n in plan["outputs"]}
+        outputs = {n: np.empty(tuple(device[n].shape), dtype=_OUTPUT_DTYPES[native.value_desc(n)[0]])
+                   for n in plan["outputs"]}
         ctx.run_host(arrays, outputs)
         return outputs

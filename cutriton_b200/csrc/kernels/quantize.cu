@@ -6,15 +6,16 @@
 // an integer. A row of zeros has s = 0 and q = 0. A row that holds an infinity
 // or a NaN has s = inf or NaN and q = 0, so that a product with it is NaN.
 //
-// One pass over HBM (3 bytes an element). A warp (two or four for long rows)
-// takes whole rows and waits for no other one: each lane copies its vectors of
-// 8 elements into a queue of its own in shared memory (cp.async), 13.5 KB a warp,
-// finds the row's maximum, and reads them back to write the integers. So 216 KB
-// of an SM's rows are under way while sixteen warps compute, which needs 10 of
-// the 16 lane instructions an element that full HBM rate leaves. (With rows in
-// registers, by blocks of 256 threads with two barriers a row, 16384x8192 ran
-// at 4.2 TB/s and 16384x2048 at 1.9; unrolled over 16 vectors a lane the code
-// outgrew the instruction cache, 1.8.)
+// One pass over HBM (3 bytes an element). A warp (two, four or eight for long
+// rows) takes whole rows and waits for no other one: each lane copies its
+// vectors of 8 elements into a queue of its own in shared memory (cp.async),
+// 9 KB a warp, finds the row's maximum, and reads them back to write the
+// integers. So 216 KB of an SM's rows are under way while 24 warps compute,
+// which takes 14 of the 16.7 lane instructions an element that full HBM rate
+// leaves: the rounding, exact by comparing two, is half of them.
+// 16384x8192: 75 us, 5.3 TB/s; 82 us with 16 warps, 85 with 12; with rows in
+// registers, by blocks of 256 threads with two barriers a row, 96 us (and
+// 16384x2048 52 us for 23).
 //
 // Element i of x and of q have the same flat index, so a vector of 8 elements
 // that starts at a multiple of 8 is 16-byte aligned in x and 8-byte aligned in
@@ -25,10 +26,10 @@
 
 namespace {
 
-constexpr int kWarps = 16;
+constexpr int kWarps = 24;
 constexpr int kThreads = kWarps * 32;
-constexpr int kSlots = 27;  // vectors of 8 elements that a lane's queue holds
-static_assert(kWarps <= 16, "row_maximum numbers its barriers by warps, from 1; there are 16");
+constexpr int kSlots = 18;  // vectors of 8 elements that a lane's queue holds
+static_assert(kWarps % 8 == 0 && kWarps / 2 < 16, "groups of two warps have a barrier each, of 15");
 constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer, half to even
 
 // Largest |x| of each FP16 half, NaN if one is.
@@ -130,13 +131,13 @@ __device__ __forceinline__ uint4 read_vector(uint32_t src) {
   return v;
 }
 
-// The maximum of a row over its `warps` warps (a power of two).
-__device__ __forceinline__ uint32_t row_maximum(uint32_t m, int warps, uint32_t* shared) {
+// The maximum of a row over the `warps` warps from `first` on, which meet at
+// `barrier` (1 to 15).
+__device__ __forceinline__ uint32_t row_maximum(uint32_t m, int first, int warps, int barrier, uint32_t* shared) {
   m = __reduce_max_sync(0xFFFFFFFFu, m);
   if (warps > 1) {
-    const int warp = threadIdx.x / 32, first = warp & ~(warps - 1), barrier = 1 + first;
     asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(32 * warps) : "memory");  // the last row's readers are done
-    if ((threadIdx.x & 31) == 0) shared[warp] = m;
+    if ((threadIdx.x & 31) == 0) shared[threadIdx.x / 32] = m;
     asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(32 * warps) : "memory");
     for (int w = 0; w < warps; ++w) m = max(m, shared[first + w]);
   }
@@ -220,7 +221,8 @@ __device__ __forceinline__ void quantize_rows(uint8_t* smem, const unsigned shor
         pair = largest(v, pair);
       }
       const uint32_t bits = *reinterpret_cast<uint32_t*>(&pair) & 0x7FFF7FFFu;
-      const uint32_t m = row_maximum(max(bits & 0xFFFFu, bits >> 16), warps, shared);
+      const uint32_t m = row_maximum(max(bits & 0xFFFFu, bits >> 16), group_in_block << warps_log2, warps,
+                                     1 + group_in_block, shared);
       const float s = scale_of(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
       if (lane == 0) scale[row0 + k] = s;
       float inv;
@@ -245,14 +247,14 @@ __device__ __forceinline__ void quantize_rows(uint8_t* smem, const unsigned shor
 }
 
 // One row by a block, element by element: tensors off 16 bytes (x) or 8 (q), and
-// rows longer than the queues of four warps.
+// rows longer than the queues of eight warps.
 __device__ __forceinline__ void quantize_row_unaligned(const unsigned short* __restrict__ x,
                                                        signed char* __restrict__ q, float* __restrict__ scale,
                                                        long long row, int columns, uint32_t* shared) {
   const unsigned short* xr = x + row * columns;
   uint32_t m = 0;
   for (int i = threadIdx.x; i < columns; i += kThreads) m = max(m, static_cast<uint32_t>(xr[i]) & 0x7FFFu);
-  m = row_maximum(m, kWarps, shared);
+  m = row_maximum(m, 0, kWarps, 1, shared);
   const float s = scale_of(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
   if (threadIdx.x == 0) scale[row] = s;
   const bool regular = m != 0 && m < 0x7C00u;
@@ -272,21 +274,24 @@ ctb_quantize_rows_f16(const unsigned short* x, signed char* q, float* scale, int
   CTB_GRID_DEPENDENCY_SYNC();
   extern __shared__ __align__(16) uint8_t smem[];
   uint32_t* shared = reinterpret_cast<uint32_t*>(smem + kWarps * kSlots * 512);
-  const int vectors = columns / 8 + 2;  // at most: a row may begin and end inside a vector
-  if (!ctb::aligned16(x) || (reinterpret_cast<uintptr_t>(q) & 7u) != 0 || vectors > 4 * 32 * kSlots) {
+  // At most: a row of a length that 8 does not divide may begin inside a vector.
+  const int vectors = columns % 8 == 0 ? columns / 8 : (columns + 14) / 8;
+  if (!ctb::aligned16(x) || (reinterpret_cast<uintptr_t>(q) & 7u) != 0 || vectors > 8 * 32 * kSlots) {
     for (int row = blockIdx.x; row < rows; row += gridDim.x) quantize_row_unaligned(x, q, scale, row, columns, shared);
     return;
   }
-  // One warp where two rows fit its queue; four where rows are few (latency
-  // counts, not rate).
-  const bool few = rows <= static_cast<int>(gridDim.x) * (kWarps / 4) && vectors > 64;
-  const int warps_log2 = few || vectors > 64 * (kSlots / 2) ? 2 : vectors > 32 * (kSlots / 2) ? 1 : 0;
+  // As many warps as two rows fit the queues of; eight where rows are few
+  // (latency counts, not rate).
+  const bool few = rows <= static_cast<int>(gridDim.x) * (kWarps / 8);
+  int warps_log2 = few ? 3 : 0;
+  while (warps_log2 < 3 && vectors > (16 << warps_log2) * kSlots) ++warps_log2;
+  while (warps_log2 > 0 && vectors <= (16 << warps_log2)) --warps_log2;
   const int slots = (vectors + (32 << warps_log2) - 1) >> (5 + warps_log2);
   if (slots > kSlots / 2) {
     quantize_rows<1>(smem, x, q, scale, rows, columns, warps_log2, slots, 1, shared);
   } else if (slots > kSlots / 4) {
     quantize_rows<2>(smem, x, q, scale, rows, columns, warps_log2, slots, 1, shared);
   } else {
-    quantize_rows<4>(smem, x, q, scale, rows, columns, warps_log2, slots, kSlots / 4 / slots, shared);
+    quantize_rows<4>(smem, x, q, scale, rows, columns, warps_log2, slots, few ? 1 : kSlots / 4 / slots, shared);
   }
 }

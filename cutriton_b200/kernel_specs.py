@@ -629,7 +629,7 @@ def _product_specs() -> list[KernelSpec]:
                       Variant("rows16_turned", arg_overrides=stream_turned,
                               constraints=(by_columns, *({"kind": "input_is_constant", "index": i} for i in weights)),
                               **stream))))
-    # One block of sixteen warps an SM: a queue of 13.5 KB a warp, and its maxima.
+    # One block of 24 warps an SM: a queue of 9 KB a warp, and its maxima.
     specs.append(KernelSpec(
         kernel_id="quantize_rows.fp16", op_type="QuantizeRows", version=1, source="quantize.cu",
         symbol="ctb_quantize_rows_f16", dtype="int8",
@@ -637,7 +637,7 @@ def _product_specs() -> list[KernelSpec]:
                    arg("scale", "*fp32", "output", index=1), arg("rows", "i32", "input_dim", index=0, axis=0),
                    arg("columns", "i32", "input_dim", index=0, axis=1)) + RESERVED,
         grid=({"kind": "min", "args": [{"kind": "input_dim", "index": 0, "axis": 0}, {"kind": "sm_count"}]},),
-        variants=(Variant("row_queues", num_warps=16, shared_memory_bytes=16 * 27 * 512 + 64, default=True, programmatic_launch=True),)))
+        variants=(Variant("row_queues", num_warps=24, shared_memory_bytes=24 * 18 * 512 + 96, default=True, programmatic_launch=True),)))
     return specs
 
 

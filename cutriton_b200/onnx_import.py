@@ -14,7 +14,7 @@ of the ONNX messages it uses directly (field numbers of onnx.proto):
 
 Besides the structure the reference's facade extracts (python/cutriton/api.py:
 77-99: names, op types, inputs, outputs, attribute names), it keeps attribute
-values, initializers (FLOAT / FLOAT16 / INT64 tensors) and input shapes, so the
+values, initializers (FLOAT / FLOAT16 / INT64 / INT8 tensors) and input shapes, so the
 imported graph compiles to a native engine.
 """
 
@@ -27,8 +27,9 @@ from typing import Any
 import numpy as np
 
 # TensorProto.DataType values used here.
-FLOAT, INT64, FLOAT16, DOUBLE, INT32 = 1, 7, 10, 11, 6
-_NUMPY = {FLOAT: np.float32, FLOAT16: np.float16, INT64: np.int64, DOUBLE: np.float64, INT32: np.int32}
+FLOAT, INT8, INT32, INT64, FLOAT16, DOUBLE = 1, 3, 6, 7, 10, 11
+_NUMPY = {FLOAT: np.float32, FLOAT16: np.float16, INT64: np.int64, DOUBLE: np.float64, INT32: np.int32,
+          INT8: np.int8}
 
 
 class OnnxFormatError(ValueError):

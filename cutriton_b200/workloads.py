@@ -8,6 +8,10 @@
 * Transformer FFN (FP16): Gemm(x, W1) -> Gelu -> Gemm(., W2) -> Add(., x) ->
   LayerNormalization, which the passes fuse into GemmGelu, Gemm and
   SkipLayerNormalization.
+* Gated FFN of language models (FP16): Gemm(x, Wgate) -> Silu, times
+  Gemm(x, Wup), -> Gemm(., Wdown) -> Add(., x) -> LayerNormalization, fused
+  into GatedGemm, Gemm and SkipLayerNormalization; and the same block on 8-bit
+  operands (QuantizeRows, QGatedGemm, QuantizeRows, QGemm).
 
 Weights come in two flavours: ``"baseline"`` — the seeded distributions of
 the benchmark configs (Kaiming-normal fan_out convs; BN gamma ~ U(0.5, 1.5),
@@ -184,6 +188,73 @@ def build_ffn(weights: dict[str, np.ndarray], tokens: int, hidden: int, inner: i
     model.add_node("residual_add", "Add", ["contracted", "x"], ["sum"])
     model.add_node("output_norm", "LayerNormalization", ["sum", "gamma", "beta"], ["output"], axis=-1, epsilon=1e-5)
     model.add_output("output")
+    return model
+
+
+def gated_ffn_weights(hidden: int, inner: int, seed: int = 0) -> dict[str, np.ndarray]:
+    """Weights [in, out] of the gated block, normal with the variance that
+    keeps unit activations at unit size."""
+    rng = np.random.default_rng(seed)
+
+    def normal(rows: int, columns: int) -> np.ndarray:
+        return (rng.standard_normal((rows, columns), dtype=np.float32) / np.float32(math.sqrt(rows))).astype(np.float16)
+
+    return {"w_gate": normal(hidden, inner), "w_up": normal(hidden, inner), "w_down": normal(inner, hidden),
+            "gamma": np.ones(hidden, np.float16), "beta": np.zeros(hidden, np.float16)}
+
+
+def quantize_weight(weight: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+    """[in, out] FP16 weight -> int8 rows by output channel [out, in] and their
+    scales (max |w| / 127, FP32); a channel of zeros has scale 0."""
+    rows = np.ascontiguousarray(weight.T).astype(np.float32)
+    scale = (np.abs(rows).max(axis=1).astype(np.float64) / 127.0).astype(np.float32)
+    safe = np.where(scale > 0, scale, np.float32(1.0))
+    return np.rint(rows.astype(np.float64) / safe.astype(np.float64)[:, None]).astype(np.int8), scale
+
+
+def _gated_ffn_input(model: Model, weights: dict[str, np.ndarray], tokens: int) -> None:
+    model.add_input("x", [tokens, weights["w_down"].shape[1]], dtype=np.float16, layout="")
+    model.add_constant("gamma", weights["gamma"], layout="")
+    model.add_constant("beta", weights["beta"], layout="")
+
+
+def _gated_ffn_tail(model: Model) -> None:
+    model.add_node("residual_add", "Add", ["contracted", "x"], ["sum"])
+    model.add_node("output_norm", "LayerNormalization", ["sum", "gamma", "beta"], ["output"], axis=-1, epsilon=1e-5)
+    model.add_output("output")
+
+
+def build_gated_ffn(weights: dict[str, np.ndarray], tokens: int, activation: str = "Silu") -> Model:
+    """`tokens` < 1 leaves the row count to shape profiles."""
+    model = Model()
+    _gated_ffn_input(model, weights, tokens)
+    for name in ("w_gate", "w_up", "w_down"):
+        model.add_constant(name, weights[name], layout="")
+    model.add_node("gate_projection", "Gemm", ["x", "w_gate"], ["gate"])
+    model.add_node("activation", activation, ["gate"], ["activated"])
+    model.add_node("up_projection", "Gemm", ["x", "w_up"], ["up"])
+    model.add_node("gating", "Mul", ["activated", "up"], ["gated"])
+    model.add_node("down_projection", "Gemm", ["gated", "w_down"], ["contracted"])
+    _gated_ffn_tail(model)
+    return model
+
+
+def build_gated_ffn_int8(weights: dict[str, np.ndarray], tokens: int, activation: int = 0) -> Model:
+    """The block with 8-bit weights (a scale for each output channel) and
+    activations (a scale for each token); `activation`: 0 SiLU, 1 erf-GELU."""
+    model = Model()
+    _gated_ffn_input(model, weights, tokens)
+    for name in ("gate", "up", "down"):
+        rows, scale = quantize_weight(weights["w_" + name])
+        model.add_constant("w_" + name, rows, layout="")
+        model.add_constant(name + "_scale", scale, layout="")
+    model.add_node("quantize_input", "QuantizeRows", ["x"], ["x8", "x_scale"])
+    model.add_node("gated_projection", "QGatedGemm",
+                   ["x8", "x_scale", "w_gate", "gate_scale", "w_up", "up_scale"], ["gated"], activation=activation,
+                   transB=1)
+    model.add_node("quantize_inner", "QuantizeRows", ["gated"], ["h8", "h_scale"])
+    model.add_node("down_projection", "QGemm", ["h8", "h_scale", "w_down", "down_scale"], ["contracted"], transB=1)
+    _gated_ffn_tail(model)
     return model
 
 

@@ -150,3 +150,146 @@ def test_square_of_one_projection_is_not_a_gated_pair():
     model.add_node("product", "Mul", ["a", "g"], ["y"])
     model.add_output("y")
     assert [op["op_type"] for op in ct.build_engine(model).ops()] == ["Gemm", "Silu", "Mul"]
+
+
+def test_few_row_form_is_a_candidate_of_every_plan():
+    """Its row limit holds or not at a run's shapes, so lowering admits it and
+    keeps the default; unfused steps never use it."""
+    engine = ct.build_engine(ff.product_graph("QGemm", zeros(**QGEMM), transB=1))
+    (op,) = engine.ops()
+    assert any(".stream:" in c for c in op["candidates"])
+    assert ".pair:" in op["candidates"][op["default"]]
+
+
+@pytest.mark.parametrize("k", [31, 17])
+def test_inner_sizes_off_16_bytes_take_the_general_form(k):
+    shapes = {n: (d, tuple(k if e == 32 else e for e in s)) for n, (d, s) in QGEMM.items()}
+    (op,) = ct.build_engine(ff.product_graph("QGemm", zeros(**shapes), transB=1)).ops()
+    assert len(op["candidates"]) == 1 and ".any:" in op["candidates"][0]
+
+
+def test_at_run_constraint_is_part_of_the_pack_schema():
+    from cutriton_b200 import kernel_sdk, kernel_specs
+
+    specs = [s for s in kernel_specs.all_specs() if s.kernel_id.endswith(".stream")]
+    assert len(specs) == 3
+    for spec in specs:
+        assert any(c.get("at_run") == 1 and c["value"] == 16 for c in spec.constraints)
+        kernel_sdk.KernelSpec.validate(spec)
+
+
+def test_launch_shapes_match_the_kernels():
+    """Block sizes, shared memory and boxes that the pack gives and the kernels
+    were compiled for."""
+    import re
+    from pathlib import Path
+
+    from cutriton_b200 import kernel_specs
+
+    folder = Path(kernel_specs.__file__).resolve().parent / "csrc" / "kernels"
+
+    def constant(source, name):
+        return int(re.search(rf"constexpr (?:int|uint32_t) {name} = (\d+);", (folder / source).read_text()).group(1))
+
+    for spec in kernel_specs.all_specs():
+        for variant in spec.variants:
+            if spec.source == "product_pair.cu":
+                assert variant.num_warps == 2 + constant(spec.source, "kEpilogueWarps")
+                boxes = {a.name: a.source["box"] for a in spec.arguments if a.source["kind"] == "tensor_map"}
+                block = 64 if ".fp16." in spec.kernel_id else 128
+                assert [boxes[f"tma_x{r}"] for r in (128, 64, 32)] == [[block, r] for r in (128, 64, 32)]
+                for name in ("w",) if spec.op_type == "QGemm" else ("gate", "up"):
+                    assert [boxes[f"tma_{name}{r}"] for r in (128, 96, 64, 48, 32)] == \
+                        [[block, r] for r in (128, 96, 64, 48, 32)]
+                need = constant(spec.source, "kRingBytes") + 16 * 32 * 32 * 2 + 200 + 1024
+                assert need <= variant.shared_memory_bytes <= 232448
+            elif spec.source == "product_stream.cu":
+                assert variant.num_warps == constant(spec.source, "kWarps") + constant(spec.source, "kJoinWarps")
+                assert variant.shared_memory_bytes == constant(spec.source, "kSharedBytes") <= 232448
+            elif spec.source == "quantize.cu":
+                warps = constant(spec.source, "kWarps")
+                assert variant.num_warps == warps
+                assert variant.shared_memory_bytes >= warps * (constant(spec.source, "kSlots") * 512 + 4)
+
+
+def test_workload_blocks_lower_to_the_operators():
+    from cutriton_b200 import workloads
+
+    weights = workloads.gated_ffn_weights(64, 160)
+    assert [o["op_type"] for o in ct.build_engine(workloads.build_gated_ffn(weights, 5)).ops()] == \
+        ["GatedGemm", "Gemm", "SkipLayerNormalization"]
+    assert [o["op_type"] for o in ct.build_engine(workloads.build_gated_ffn_int8(weights, 5)).ops()] == \
+        ["QuantizeRows", "QGatedGemm", "QuantizeRows", "QGemm", "SkipLayerNormalization"]
+
+
+def test_quantized_weight_holds_its_values():
+    from cutriton_b200 import workloads
+
+    weight = workloads.gated_ffn_weights(48, 40)["w_gate"]
+    weight[:, 7] = 0
+    rows, scale = workloads.quantize_weight(weight)
+    assert rows.dtype == np.int8 and rows.shape == (40, 48) and scale[7] == 0 and not rows[7].any()
+    # Half a step of the channel's scale (and the scale's own rounding).
+    error = np.abs(rows * scale.astype(np.float64)[:, None] - weight.T.astype(np.float64))
+    assert (error <= scale[:, None] * (0.5 + 128 * 2.0**-24)).all()
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", 0, 1])
+def test_facade_takes_the_operators(tmp_path, activation):
+    import json
+
+    from cutriton_b200 import api
+
+    graph = {"inputs": ["x"], "outputs": ["y"], "input_shapes": {"x": [-1, 16]}, "input_dtypes": {"x": "float16"},
+             "nodes": [{"name": "q", "op_type": "QuantizeRows", "inputs": ["x"], "outputs": ["x8", "xs"]},
+                       {"name": "g", "op_type": "QGatedGemm", "inputs": ["x8", "xs", "wg", "gs", "wu", "us"],
+                        "outputs": ["y"], "activation": activation, "transB": 1}],
+             "constants": {**{n: {"data": [1] * 128, "shape": [8, 16], "dtype": "int8"} for n in ("wg", "wu")},
+                           **{n: {"data": [0.5] * 8, "shape": [8], "dtype": "float32"} for n in ("gs", "us")}}}
+    path = tmp_path / "g.json"
+    path.write_text(json.dumps(graph))
+    native = api.compile(path).native({"x": (3, 16)})
+    assert [o["op_type"] for o in native.ops()] == ["QuantizeRows", "QGatedGemm"]
+    assert native.value_desc("y") == (ct.FLOAT16, (3, 8))
+
+
+def test_facade_refuses_other_activations(tmp_path):
+    import json
+
+    from cutriton_b200 import api
+
+    graph = {"inputs": ["x", "a", "b"], "outputs": ["y"], "input_dtypes": {n: "float16" for n in "xab"},
+             "nodes": [{"name": "g", "op_type": "GatedGemm", "inputs": ["x", "a", "b"], "outputs": ["y"],
+                        "activation": "tanh"}]}
+    path = tmp_path / "g.json"
+    path.write_text(json.dumps(graph))
+    with pytest.raises(api.UnsupportedModelError):
+        api.compile(path).native({"x": (3, 16), "a": (16, 8), "b": (16, 8)})
+
+
+def test_scale_without_a_reader_is_planned():
+    model = ct.Model()
+    model.add_input("x", [4, 32], dtype=np.float16, layout="")
+    model.add_node("quantize", "QuantizeRows", ["x"], ["q", "unused"])
+    model.add_output("q")
+    engine = ct.build_engine(model)
+    assert engine.workspace_bytes() >= 16
+
+
+def test_quantize_rows_needs_both_outputs():
+    model = ct.Model()
+    model.add_input("x", [4, 32], dtype=np.float16, layout="")
+    model.add_node("quantize", "QuantizeRows", ["x"], ["q"])
+    model.add_output("q")
+    with pytest.raises(ct.CutritonError) as error:
+        ct.build_engine(model)
+    assert error.value.code == ct.SHAPE_ERROR
+
+
+def test_one_matrix_may_be_both_weights():
+    model = ct.Model()
+    model.add_input("x", [4, 32], dtype=np.float16, layout="")
+    model.add_constant("w", np.zeros((24, 32), np.float16), layout="")
+    model.add_node("node", "GatedGemm", ["x", "w", "w"], ["y"], transB=1)
+    model.add_output("y")
+    assert ct.build_engine(model).value_desc("y") == (ct.FLOAT16, (4, 24))

@@ -257,3 +257,293 @@ def test_unaligned_tensors(cuda):
     np.testing.assert_array_equal(q[1:x.size + 1].cpu().numpy().reshape(x.shape), want_q)
     np.testing.assert_array_equal(scale.cpu().numpy(), want_scale)
     assert q[0] == 77 and (q[x.size + 1:] == 77).all()
+
+
+def test_quantize_rows_every_maximum(cuda):
+    """Every finite FP16 magnitude as a row's largest: the scale is the
+    rounded quotient for each."""
+    x = np.zeros((0x7C00, 12), np.float16)
+    x[:, 5] = np.arange(0x7C00, dtype=np.uint16).view(np.float16)
+    x[:, 7] = -x[:, 5] / 2
+    check_quantize(x)
+
+
+def single(op, inputs, constants=(), **attributes):
+    """The outputs of one node run by itself, on the device."""
+    import torch
+
+    engine = ct.build_engine(ff.product_graph(op, {**{n: _host(t) for n, t in inputs.items()}}, constants, **attributes),
+                             tuning_mode=ct.TUNING_DISABLED)
+    context = engine.create_context()
+    for name, tensor in inputs.items():
+        if name not in constants:
+            context.bind_tensor(name, tensor)
+    names = ["q", "q_scale"] if op == "QuantizeRows" else ["y"]
+    outputs = []
+    for name in names:
+        code, shape = engine.value_desc(name)
+        dtype = {ct.FLOAT16: torch.float16, ct.FLOAT32: torch.float32, ct.INT8: torch.int8}[code]
+        outputs.append(torch.empty(shape, dtype=dtype, device="cuda"))
+        context.bind_tensor(name, outputs[-1], output=True)
+    torch.cuda.synchronize()
+    context.run()
+    return outputs
+
+
+def _host(tensor):
+    return tensor if isinstance(tensor, np.ndarray) else tensor.cpu().numpy()
+
+
+def run_block(model, x, candidates=None, **options):
+    import torch
+
+    engine = ct.build_engine(model, tuning_mode=ct.TUNING_DISABLED, **options)
+    context = engine.create_context()
+    context.bind_tensor("x", x)
+    y = torch.full_like(x, 77)
+    context.bind_tensor("output", y, output=True)
+    torch.cuda.synchronize()
+    context.run()
+    return y, engine, context
+
+
+@pytest.mark.parametrize("tokens", [1, 16, 17, 300])
+def test_8bit_block_is_its_steps(cuda, tokens):
+    """Quantise, gated product, quantise, down projection, residual and norm in
+    one graph: bit for bit what the operators give one after another."""
+    import torch
+
+    from cutriton_b200 import workloads
+
+    weights = workloads.gated_ffn_weights(192, 528, seed=2)
+    x = torch.from_numpy(workloads.ffn_input(tokens, 192, seed=3)).cuda()
+    y, _, _ = run_block(workloads.build_gated_ffn_int8(weights, tokens), x)
+    eight = {name: workloads.quantize_weight(weights["w_" + name]) for name in ("gate", "up", "down")}
+    dev = {f"{n}{i}": torch.from_numpy(a).cuda() for n, pair in eight.items() for i, a in enumerate(pair)}
+    x8, x_scale = single("QuantizeRows", {"x": x})
+    (h,) = single("QGatedGemm", {"x": x8, "x_scale": x_scale, "w_gate": dev["gate0"], "gate_scale": dev["gate1"],
+                                 "w_up": dev["up0"], "up_scale": dev["up1"]}, transB=1)
+    h8, h_scale = single("QuantizeRows", {"x": h})
+    (down,) = single("QGemm", {"x": h8, "x_scale": h_scale, "w": dev["down0"], "w_scale": dev["down1"]}, transB=1)
+    gamma, beta = (torch.from_numpy(weights[n]).cuda() for n in ("gamma", "beta"))
+    (want,) = single("SkipLayerNormalization", {"a": down, "x": x, "gamma": gamma, "beta": beta}, epsilon=1e-5, axis=-1)
+    assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("activation", ["Silu", "Gelu"])
+@pytest.mark.parametrize("tokens", [3, 130])
+def test_gated_block_is_its_steps(cuda, tokens, activation):
+    import torch
+
+    from cutriton_b200 import workloads
+
+    weights = workloads.gated_ffn_weights(128, 336, seed=4)
+    x = torch.from_numpy(workloads.ffn_input(tokens, 128, seed=5)).cuda()
+    y, engine, _ = run_block(workloads.build_gated_ffn(weights, tokens, activation), x)
+    assert engine.op(0)["op_type"] == "GatedGemm"
+    constants = {"x": x, "w_gate": weights["w_gate"], "w_up": weights["w_up"]}
+    (h,) = single("GatedGemm", constants, ("w_gate", "w_up"), activation=0 if activation == "Silu" else 1)
+    (down,) = single("Gemm", {"x": h, "w": weights["w_down"]}, ("w",))
+    gamma, beta = (torch.from_numpy(weights[n]).cuda() for n in ("gamma", "beta"))
+    (want,) = single("SkipLayerNormalization", {"a": down, "x": x, "gamma": gamma, "beta": beta}, epsilon=1e-5, axis=-1)
+    assert torch.equal(y, want)
+
+
+def test_row_counts_of_one_profile_choose_their_form(cuda):
+    """One engine over 1 to 400 tokens: each run equals a static engine of its
+    shape, at most 16 rows take the few-row form, captured graphs are kept."""
+    import torch
+
+    from cutriton_b200 import workloads
+
+    weights = workloads.gated_ffn_weights(128, 272, seed=6)
+    model = workloads.build_gated_ffn_int8(weights, -1)
+    model.add_shape_profile("tokens", "x", [1, 128], [64, 128], [400, 128])
+    engine = ct.build_engine(model, tuning_mode=ct.TUNING_DISABLED)
+    context = engine.create_context()
+    ops = engine.ops()
+    gated = [o["op_type"] for o in ops].index("QGatedGemm")
+    for tokens in (64, 1, 16, 17, 400, 16, 1):
+        x = torch.from_numpy(workloads.ffn_input(tokens, 128, seed=tokens)).cuda()
+        y = torch.empty_like(x)
+        context.set_input_shape("x", [tokens, 128])
+        context.resolve_shapes()
+        context.bind_tensor("x", x)
+        context.bind_tensor("output", y, output=True)
+        torch.cuda.synchronize()
+        context.run()
+        chosen = ops[gated]["candidates"][context.selected_candidate(gated)]
+        assert (".stream:" in chosen) == (tokens <= 16), (tokens, chosen)
+        want, _, _ = run_block(workloads.build_gated_ffn_int8(weights, tokens), x)
+        assert torch.equal(y, want), tokens
+    assert context.cached_graph_count() >= 2
+
+
+def test_replays_and_streams_give_the_same(cuda):
+    """A captured graph replayed on changed inputs, two contexts of one engine
+    at once on two streams, and a run without graphs."""
+    import torch
+
+    from cutriton_b200 import workloads
+
+    weights = workloads.gated_ffn_weights(256, 624, seed=8)
+    for tokens in (9, 200):
+        xs = [torch.from_numpy(workloads.ffn_input(tokens, 256, seed=s)).cuda() for s in range(6)]
+        engine = ct.build_engine(workloads.build_gated_ffn_int8(weights, tokens), tuning_mode=ct.TUNING_DISABLED)
+        contexts = [engine.create_context() for _ in range(2)]
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        bound = [(torch.empty_like(xs[0]), torch.empty_like(xs[0])) for _ in range(2)]
+        for context, (x, y) in zip(contexts, bound):
+            context.bind_tensor("x", x)
+            context.bind_tensor("output", y, output=True)
+        got = []
+        for i in range(0, 6, 2):
+            for j in range(2):
+                bound[j][0].copy_(xs[i + j])
+            torch.cuda.synchronize()
+            for j in range(2):
+                contexts[j].run_async(streams[j].cuda_stream)
+            for j in range(2):
+                contexts[j].synchronize()
+                got.append(bound[j][1].clone())
+        for x, y in zip(xs, got):
+            want, _, _ = run_block(workloads.build_gated_ffn_int8(weights, tokens), x, enable_cuda_graph=0)
+            assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("rows", [4, 40])
+def test_tuner_chooses_among_the_forms_that_take_the_shape(cuda, tmp_path, rows):
+    rng = np.random.default_rng(9)
+    inputs = ff.qgemm_case(rng, rows, 256, 96, True)
+    runner = Runner(ff.product_graph("QGemm", inputs, transB=1), inputs, tuning_mode=ct.TUNING_TUNE_ON_MISS,
+                    tuning_cache_dir=str(tmp_path))
+    runner.output("y", (rows, 96), np.float16)
+    ff.assert_within(runner.run()["y"], ff.qgemm_result(inputs), "tuned")
+    chosen = runner.engine.op(0)["candidates"][runner.context.selected_candidate(0)]
+    assert rows <= 16 or ".stream:" not in chosen
+    assert len(list(tmp_path.glob("*.json"))) == 1
+
+
+def test_facade_runs_the_8bit_pair(cuda, tmp_path):
+    import json
+
+    from cutriton_b200 import api
+
+    rng = np.random.default_rng(10)
+    w, scale = ff.quantized(rng, 24, 48)
+    graph = {"inputs": ["x"], "outputs": ["x8", "xs", "y"], "input_dtypes": {"x": "float16"},
+             "nodes": [{"name": "q", "op_type": "QuantizeRows", "inputs": ["x"], "outputs": ["x8", "xs"]},
+                       {"name": "p", "op_type": "QGemm", "inputs": ["x8", "xs", "w", "ws"], "outputs": ["y"],
+                        "transB": 1}],
+             "constants": {"w": {"data": w.ravel().tolist(), "shape": [24, 48], "dtype": "int8"},
+                           "ws": {"data": scale.tolist(), "shape": [24], "dtype": "float32"}}}
+    path = tmp_path / "g.json"
+    path.write_text(json.dumps(graph))
+    context = api.compile(path).create_context()
+    for rows in (2, 30):
+        x = rng.standard_normal((rows, 48)).astype(np.float16)
+        got = context.run({"x": x})
+        q, q_scale = ff.quantize_result(x)
+        np.testing.assert_array_equal(got["x8"], q)
+        np.testing.assert_array_equal(got["xs"], q_scale)
+        ff.assert_within(got["y"], ff.qgemm_result({"x": q, "x_scale": q_scale, "w": w, "w_scale": scale}), "facade")
+
+
+@pytest.mark.parametrize("rows", [3, 50])
+def test_products_off_16_bytes_fail_with_an_error(cuda, rows):
+    """An activation bound off 16 bytes: an error, and the context goes on."""
+    import torch
+
+    rng = np.random.default_rng(12)
+    inputs = ff.gated_case(rng, rows, 64, 40)
+    engine = ct.build_engine(ff.product_graph("GatedGemm", inputs, transB=1), tuning_mode=ct.TUNING_DISABLED,
+                             enable_cuda_graph=0)
+    context = engine.create_context()
+    device = {n: torch.from_numpy(a).cuda() for n, a in inputs.items()}
+    shifted = torch.zeros(rows * 64 + 1, dtype=torch.float16, device="cuda")
+    shifted[1:] = device["x"].reshape(-1)
+    y = torch.empty(rows, 40, dtype=torch.float16, device="cuda")
+    for name in ("w_gate", "w_up"):
+        context.bind_tensor(name, device[name])
+    context.bind_tensor("x", shifted[1:])
+    context.bind_tensor("y", y, output=True)
+    torch.cuda.synchronize()
+    with pytest.raises(ct.CutritonError) as error:
+        context.run()
+    assert error.value.code == ct.RUNTIME_ERROR
+    context.bind_tensor("x", device["x"])
+    context.run()
+    ff.assert_within(y.cpu().numpy(), ff.gated_result(inputs, 0), "after the error")
+
+
+@pytest.mark.parametrize("shape", [(1, 5), (33, 250), (700, 1000)], ids=str)
+def test_silu_and_mul(cuda, shape):
+    """The unfused steps: SiLU in FP32 (2^-18 relative for the exponential and
+    the division) rounded once, the product in FP16 as numpy's."""
+    rng = np.random.default_rng(shape)
+    x = (rng.standard_normal(shape) * 8).astype(np.float16)
+    x.flat[:5] = [0, -0.0, 65504, -65504, 2.0**-24]
+    y = rng.standard_normal(shape).astype(np.float16)
+    model = ct.Model()
+    for name in "xy":
+        model.add_input(name, list(shape), dtype=np.float16, layout="")
+    model.add_node("silu", "Silu", ["x"], ["s"])
+    model.add_node("mul", "Mul", ["x", "y"], ["m"])
+    model.add_output("s")
+    model.add_output("m")
+    runner = Runner(model, {"x": x, "y": y})
+    runner.output("s", shape, np.float16)
+    runner.output("m", shape, np.float16)
+    got = runner.run()
+    want = ff.activate(x.astype(np.float64), ff.SILU)
+    tol = (2.0**-18 + ff.HALF) * np.abs(want) + ff.HALF_MIN
+    assert (np.abs(got["s"].astype(np.float64) - want) <= tol).all()
+    np.testing.assert_array_equal(got["m"], x * y)
+
+
+def test_offsets_past_32_bits(cuda):
+    """More than 2^31 elements in a quantised matrix and in a product's output."""
+    import torch
+
+    rows, columns = 524300, 4097
+    x = torch.empty(rows, columns, dtype=torch.float16, device="cuda")
+    x.normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    q, scale = single_on_device("QuantizeRows", {"x": x})
+    for part in (slice(0, 3), slice(rows // 2, rows // 2 + 3), slice(rows - 3, rows)):
+        want_q, want_scale = ff.quantize_result(x[part].cpu().numpy())
+        np.testing.assert_array_equal(q[part].cpu().numpy(), want_q)
+        np.testing.assert_array_equal(scale[part].cpu().numpy(), want_scale)
+    del x, q, scale
+    m, n, k = 70001, 32769, 48
+    rng = np.random.default_rng(2)
+    inputs = ff.gated_case(rng, m, k, n)
+    (y,) = single_on_device("GatedGemm", {name: torch.from_numpy(a).cuda() for name, a in inputs.items()}, transB=1)
+    for part in (slice(0, 2), slice(m // 2, m // 2 + 2), slice(m - 2, m)):
+        ff.assert_within(y[part].cpu().numpy(), ff.gated_result({**inputs, "x": inputs["x"][part]}, 0), "far rows")
+
+
+def single_on_device(op, tensors, **attributes):
+    """One node over device tensors, without host copies of them."""
+    import torch
+
+    names = {torch.float16: "float16", torch.int8: "int8", torch.float32: "float32"}
+    model = ct.Model()
+    for name, t in tensors.items():
+        model.add_input(name, list(t.shape), dtype=names[t.dtype], layout="")
+    outs = ["q", "q_scale"] if op == "QuantizeRows" else ["y"]
+    model.add_node("node", op, list(tensors), outs, **attributes)
+    for name in outs:
+        model.add_output(name)
+    engine = ct.build_engine(model, tuning_mode=ct.TUNING_DISABLED)
+    context = engine.create_context()
+    for name, t in tensors.items():
+        context.bind_tensor(name, t)
+    outputs = []
+    for name in outs:
+        code, shape = engine.value_desc(name)
+        dtype = {ct.FLOAT16: torch.float16, ct.FLOAT32: torch.float32, ct.INT8: torch.int8}[code]
+        outputs.append(torch.empty(shape, dtype=dtype, device="cuda"))
+        context.bind_tensor(name, outputs[-1], output=True)
+    torch.cuda.synchronize()
+    context.run()
+    return outputs
