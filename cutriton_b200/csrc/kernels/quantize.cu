@@ -13,7 +13,7 @@
 // integers. So 216 KB of an SM's rows are under way while 24 warps compute,
 // which takes 14 of the 16.7 lane instructions an element that full HBM rate
 // leaves: the rounding, exact by comparing two, is half of them.
-// 16384x8192: 75 us, 5.3 TB/s; 82 us with 16 warps, 85 with 12; with rows in
+// 16384x8192: 67 us, 6.0 TB/s (with 16 warps 9 %, with 12 13 % more); with rows in
 // registers, by blocks of 256 threads with two barriers a row, 96 us (and
 // 16384x2048 52 us for 23).
 //
@@ -164,16 +164,16 @@ __device__ __forceinline__ Row row_at(const unsigned short* x, signed char* q, l
 }
 
 // Batches of `batch` rows of `slots` vectors a lane, kAhead batches in the
-// queue, by groups of `warps` warps.
-template <int kAhead>
+// queue, by groups of 2^kWarpsLog2 warps (with the number of warps known to the
+// compiler 16384x8192 takes 67 us instead of 75).
+template <int kWarpsLog2, int kAhead>
 __device__ __forceinline__ void quantize_rows(uint8_t* smem, const unsigned short* __restrict__ x,
                                               signed char* __restrict__ q, float* __restrict__ scale, int rows,
-                                              int columns, int warps_log2, int slots, int batch,
-                                              uint32_t* shared) {
-  const int warps = 1 << warps_log2, lanes_log2 = 5 + warps_log2, lanes = 1 << lanes_log2;
-  const int group_in_block = threadIdx.x >> lanes_log2;
-  const int lane = threadIdx.x & (lanes - 1);
-  const int groups_a_block = kWarps >> warps_log2;
+                                              int columns, int slots, int batch, uint32_t* shared) {
+  constexpr int kGroupWarps = 1 << kWarpsLog2, kLanesLog2 = 5 + kWarpsLog2, kLanes = 1 << kLanesLog2;
+  const int group_in_block = threadIdx.x >> kLanesLog2;
+  const int lane = threadIdx.x & (kLanes - 1);
+  constexpr int groups_a_block = kWarps >> kWarpsLog2;
   const long long groups = static_cast<long long>(gridDim.x) * groups_a_block;
   const long long group = static_cast<long long>(blockIdx.x) * groups_a_block + group_in_block;
   const long long total = static_cast<long long>(rows) * columns;
@@ -190,10 +190,10 @@ __device__ __forceinline__ void quantize_rows(uint8_t* smem, const unsigned shor
       const long long end = (fetch + k) * columns - r.head + 8ll * r.vectors;
       const int last_bytes = end > total ? 16 - 2 * static_cast<int>(end - total) : 16;
       const uint32_t dst = queue + place * batch_bytes + static_cast<uint32_t>(k * slots) * 512;
-      const int mine = lane < r.vectors ? ((r.vectors - lane - 1) >> lanes_log2) + 1 : 0;
+      const int mine = lane < r.vectors ? ((r.vectors - lane - 1) >> kLanesLog2) + 1 : 0;
 #pragma unroll 4
       for (int j = 0; j < mine; ++j) {
-        const int i = (j << lanes_log2) + lane;
+        const int i = (j << kLanesLog2) + lane;
         copy_vector(dst + j * 512, r.x + i, i == r.vectors - 1 ? last_bytes : 16);
       }
     }
@@ -212,16 +212,16 @@ __device__ __forceinline__ void quantize_rows(uint8_t* smem, const unsigned shor
       const bool ragged = r.head != 0 || r.tail != 8;
       const uint32_t src = queue + at * batch_bytes + static_cast<uint32_t>(k * slots) * 512;
       __half2 pair = __half2half2(__ushort_as_half(0));
-      const int mine = lane < r.vectors ? ((r.vectors - lane - 1) >> lanes_log2) + 1 : 0;
+      const int mine = lane < r.vectors ? ((r.vectors - lane - 1) >> kLanesLog2) + 1 : 0;
 #pragma unroll 4
       for (int j = 0; j < mine; ++j) {
-        const int i = (j << lanes_log2) + lane;
+        const int i = (j << kLanesLog2) + lane;
         uint4 v = read_vector(src + j * 512);
         if (ragged && (i == 0 || i == r.vectors - 1)) v = trimmed(r, i, v);
         pair = largest(v, pair);
       }
       const uint32_t bits = *reinterpret_cast<uint32_t*>(&pair) & 0x7FFF7FFFu;
-      const uint32_t m = row_maximum(max(bits & 0xFFFFu, bits >> 16), group_in_block << warps_log2, warps,
+      const uint32_t m = row_maximum(max(bits & 0xFFFFu, bits >> 16), group_in_block << kWarpsLog2, kGroupWarps,
                                      1 + group_in_block, shared);
       const float s = scale_of(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
       if (lane == 0) scale[row0 + k] = s;
@@ -230,7 +230,7 @@ __device__ __forceinline__ void quantize_rows(uint8_t* smem, const unsigned shor
       const bool regular = m != 0 && m < 0x7C00u;
 #pragma unroll 4
       for (int j = 0; j < mine; ++j) {
-        const int i = (j << lanes_log2) + lane;
+        const int i = (j << kLanesLog2) + lane;
         const uint2 packed = regular ? quantize(read_vector(src + j * 512), s, inv) : make_uint2(0, 0);
         if (ragged && (i == 0 || i == r.vectors - 1)) {
           store_elements(r, i, packed);
@@ -280,18 +280,36 @@ ctb_quantize_rows_f16(const unsigned short* x, signed char* q, float* scale, int
     for (int row = blockIdx.x; row < rows; row += gridDim.x) quantize_row_unaligned(x, q, scale, row, columns, shared);
     return;
   }
-  // As many warps as two rows fit the queues of; eight where rows are few
-  // (latency counts, not rate).
-  const bool few = rows <= static_cast<int>(gridDim.x) * (kWarps / 8);
-  int warps_log2 = few ? 3 : 0;
-  while (warps_log2 < 3 && vectors > (16 << warps_log2) * kSlots) ++warps_log2;
-  while (warps_log2 > 0 && vectors <= (16 << warps_log2)) --warps_log2;
-  const int slots = (vectors + (32 << warps_log2) - 1) >> (5 + warps_log2);
-  if (slots > kSlots / 2) {
-    quantize_rows<1>(smem, x, q, scale, rows, columns, warps_log2, slots, 1, shared);
-  } else if (slots > kSlots / 4) {
-    quantize_rows<2>(smem, x, q, scale, rows, columns, warps_log2, slots, 1, shared);
+  // Warps a row: those that finish first, by rounds of rows over the groups of
+  // warps and a row's slots plus two for its maximum, among those whose queues
+  // hold two rows (eight warps: one). 16384 rows of 2048: one warp 22 us, two
+  // 24; 2048 rows of 4096: four 9.1 us, two 10.5; 8 rows: eight.
+  int warps_log2 = 3, slots = (vectors + 255) >> 8, rounds = 1;
+  float least = INFINITY;
+#pragma unroll
+  for (int w = 3; w >= 0; --w) {
+    const int lane_vectors = (vectors + (32 << w) - 1) >> (5 + w);
+    const float turns = ceilf(__fdividef(static_cast<float>(rows), static_cast<float>(gridDim.x * (kWarps >> w))));
+    const float cost = turns * static_cast<float>(lane_vectors + 2);
+    if (cost < least && (w == 3 || lane_vectors <= kSlots / 2)) {
+      least = cost;
+      warps_log2 = w;
+      slots = lane_vectors;
+      rounds = static_cast<int>(turns);
+    }
+  }
+  if (warps_log2 == 0 && slots <= kSlots / 4) {
+    quantize_rows<0, 4>(smem, x, q, scale, rows, columns, slots,
+                         min(rounds, kSlots / 4 / slots), shared);
+  } else if (warps_log2 == 0) {
+    quantize_rows<0, 2>(smem, x, q, scale, rows, columns, slots, 1, shared);
+  } else if (warps_log2 == 1) {
+    quantize_rows<1, 2>(smem, x, q, scale, rows, columns, slots, 1, shared);
+  } else if (warps_log2 == 2) {
+    quantize_rows<2, 2>(smem, x, q, scale, rows, columns, slots, 1, shared);
+  } else if (slots <= kSlots / 2) {
+    quantize_rows<3, 2>(smem, x, q, scale, rows, columns, slots, 1, shared);
   } else {
-    quantize_rows<4>(smem, x, q, scale, rows, columns, warps_log2, slots, few ? 1 : kSlots / 4 / slots, shared);
+    quantize_rows<3, 1>(smem, x, q, scale, rows, columns, slots, 1, shared);
   }
 }

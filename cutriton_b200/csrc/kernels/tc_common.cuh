@@ -77,11 +77,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // another thread of the CTA.
 __device__ __forceinline__ bool mbar_wait_for(uint64_t* bar, uint32_t parity, volatile int* abort, void* scratch,
                                               unsigned int site, unsigned long long limit_ns) {
-  // The clock is read only when a wait has already lasted many tries: reading
-  // it costs about 500 clocks, more than most waits of a full pipeline.
-  for (int i = 0; i < 64; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-  }
+  if (mbar_try_wait(bar, parity)) return true;
   const unsigned long long start = global_time_ns();
   for (uint32_t spin = 1;; ++spin) {
     if (mbar_try_wait(bar, parity)) return true;
