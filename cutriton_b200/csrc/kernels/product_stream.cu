@@ -7,8 +7,8 @@
 // enough bytes in flight (about 45 KB an SM), not tensor throughput:
 //
 // * One CTA an SM; the CTAs share the output columns out evenly in groups of
-//   8. The 16 reading warps of a CTA take the 64-byte chunks of K in turn. A batch is four groups of weight rows (for the gated
-//   ops two of each matrix).
+//   8. The reading warps of a CTA take the 64-byte chunks of K in turn. A batch
+//   is four groups of weight rows, for the gated ops four of each matrix.
 // * A warp reads a batch's chunk of 8 rows x 64 bytes with one 16-byte
 //   cp.async a lane into a queue in shared memory that is private to the
 //   lane, so the copies need no barrier: a lane waits for its own oldest
@@ -24,7 +24,8 @@
 //   is double, so no reading warp waits for another one: when all of them met
 //   at a barrier after each batch (joined over a cluster of two CTAs, K split
 //   in 16), 16x4096x12288 took 45.7 us and the 8-bit form 29.0 us for 8 rows,
-//   against 33.7 and 18 us of the reading alone.
+//   against 36.4 and 20.3 us now.
+// 1x4096x12288 reads its 201 MB in 33.8 us, 5.96 TB/s.
 // All waits are bounded (tc_common.cuh).
 
 #include "product.cuh"
@@ -36,11 +37,10 @@ using ctb::tc::mbar_arrive;
 using ctb::tc::mbar_init;
 using ctb::tc::mbar_wait;
 
-constexpr int kWarps = 16;     // reading warps, over which K is split
-constexpr int kJoinWarps = 4;  // joining warps
-constexpr int kThreads = (kWarps + kJoinWarps) * 32;
-constexpr int kGroups = 4;   // groups of 8 weight rows a batch
-constexpr int kStride = 40;  // words a token in the join buffer (conflict-free pairs)
+constexpr int kJoinWarps = 4;
+// Threads of a block: the most reading warps of a form and the joining ones.
+constexpr int kPlainThreads = (16 + kJoinWarps) * 32;
+constexpr int kGatedThreads = (12 + kJoinWarps) * 32;
 constexpr int kSharedBytes = 231424;  // barriers, join buffers, queues
 
 struct Half {
@@ -100,10 +100,13 @@ __device__ __forceinline__ uint4 read_16(uint32_t src) {
   return v;
 }
 
-// kTokens8: groups of 8 rows of x (1 or 2).
-template <typename T, bool kGated, int kTokens8>
+// kTokens8: groups of 8 rows of x (1 or 2). kWarps: reading warps, over which K
+// is split.
+template <typename T, bool kGated, int kTokens8, int kWarps>
 __device__ __forceinline__ void product_stream(uint8_t* smem, const Operands<T>& op) {
   using Sum = typename T::Sum;
+  constexpr int kGroups = kGated ? 8 : 4;     // groups of 8 weight rows a batch
+  constexpr int kStride = 8 * kGroups + 8;    // words a token in the join buffer (conflict-free pairs)
   constexpr int kPieces = kGroups + kTokens8;  // 16-byte pieces a lane and slot
   constexpr int kSlotBytes = kPieces * 512;    // a warp's
   constexpr int kTokens = 8 * kTokens8;
@@ -111,7 +114,7 @@ __device__ __forceinline__ void product_stream(uint8_t* smem, const Operands<T>&
   constexpr int kDepth = (kSharedBytes - 128 - 8 * kJoin) / (kWarps * kSlotBytes);
   static_assert(kDepth >= 3, "queue");
   constexpr int kMTiles = (kTokens8 + 1) / 2;
-  constexpr int kChannelGroups = kGated ? kGroups / 2 : kGroups;  // output groups a batch
+  constexpr int kChannelGroups = 4;  // output groups a batch
   constexpr int kChunk = 4 * T::kPiece;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
@@ -240,45 +243,50 @@ __device__ __forceinline__ void product_stream(uint8_t* smem, const Operands<T>&
     return;
   }
 
-  // ---- joining warps: tokens j, j + 4, ...; lane = column of the batch ----
+  if (warp >= kWarps + kJoinWarps) return;
+
+  // ---- joining warps: tokens j, j + 4, ...; lane = output column of the batch ----
   const int j = warp - kWarps;
   for (int batch = 0; batch < batches; ++batch) {
     const int buffer = batch & 1;
     const bool ready = mbar_wait(&bars->full[buffer], (batch >> 1) & 1, abort, op.scratch, 82);
     __syncwarp();
     if (!ready) break;
-    Sum total[kTokens / kJoinWarps];
+    Sum total[kTokens / kJoinWarps], up[kTokens / kJoinWarps];
 #pragma unroll
     for (int r = 0; r < kTokens / kJoinWarps; ++r) {
       const int token = j + kJoinWarps * r;
-      total[r] = 0;
+      total[r] = up[r] = 0;
       if (token >= op.m) continue;
+      const Sum* src = join + buffer * kJoin + token * kStride + lane;
 #pragma unroll
-      for (int v = 0; v < kWarps; ++v) total[r] += join[buffer * kJoin + (v * kTokens + token) * kStride + lane];
+      for (int v = 0; v < kWarps; ++v) {
+        total[r] += src[v * kTokens * kStride];
+        if (kGated) up[r] += src[v * kTokens * kStride + 32];
+      }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars->empty[buffer]);
-    const long long column = (first + batch * kChannelGroups) * 8 + (kGated ? lane & 15 : lane);
-    const bool inside = column < op.n && column < last * 8;
-    float column_scale = 0.0f, bias = 0.0f;
-    if (T::kPiece == 16 && inside) {
-      column_scale = __ldg((kGated && lane >= 16 ? op.w_scale[1] : op.w_scale[0]) + column);
+    const long long column = (first + batch * kChannelGroups) * 8 + lane;
+    if (column >= op.n || column >= last * 8) continue;
+    float scale = 0.0f, up_scale = 0.0f, bias = 0.0f;
+    if (T::kPiece == 16) {
+      scale = __ldg(op.w_scale[0] + column);
+      if (kGated) up_scale = __ldg(op.w_scale[1] + column);
       if (!kGated && op.bias != nullptr) bias = __half2float(op.bias[column]);
     }
 #pragma unroll
     for (int r = 0; r < kTokens / kJoinWarps; ++r) {
       const int token = j + kJoinWarps * r;
       if (token >= op.m) continue;
-      float y = static_cast<float>(total[r]);
+      float y = static_cast<float>(total[r]), u = static_cast<float>(up[r]);
       if constexpr (T::kPiece == 16) {
-        y = ctb::dequantized(total[r], __ldg(op.x_scale + token), column_scale, bias);
+        const float row_scale = __ldg(op.x_scale + token);
+        y = ctb::dequantized(total[r], row_scale, scale, bias);
+        if (kGated) u = ctb::dequantized(up[r], row_scale, up_scale, 0.0f);
       }
-      if constexpr (kGated) {
-        const float up = __shfl_down_sync(0xFFFFFFFFu, y, 16);
-        y = ctb::gated(y, up, op.activation);
-        if (lane >= 16) continue;
-      }
-      if (inside) op.out[static_cast<long long>(token) * op.n + column] = __float2half_rn(y);
+      if (kGated) y = ctb::gated(y, u, op.activation);
+      op.out[static_cast<long long>(token) * op.n + column] = __float2half_rn(y);
     }
   }
 }
@@ -294,16 +302,19 @@ __device__ __forceinline__ void product_dispatch(const Operands<T>& op) {
     if (threadIdx.x == 0) ctb::report_error(op.scratch, ctb::kErrorBadShape, 80);
     return;
   }
+  // Reading warps: as many as leave every queue three slots and more beside
+  // the join buffers (16x4096x12288 with eight 36.4 us, with twelve 45.6).
+  constexpr int kFew = kGated ? 12 : 16, kMore = kGated ? 8 : 16;
   if (op.m <= 8) {
-    product_stream<T, kGated, 1>(smem, op);
+    product_stream<T, kGated, 1, kFew>(smem, op);
   } else {
-    product_stream<T, kGated, 2>(smem, op);
+    product_stream<T, kGated, 2, kMore>(smem, op);
   }
 }
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(kThreads, 1)
+extern "C" __global__ void __launch_bounds__(kGatedThreads, 1)
 ctb_gated_gemm_f16_stream(const __half* x, const __half* w_gate, const __half* w_up, __half* output, int m, int n,
                           int k, int activation, CTB_RESERVED_PARAMS) {
   (void)profile_scratch;
@@ -312,7 +323,7 @@ ctb_gated_gemm_f16_stream(const __half* x, const __half* w_gate, const __half* w
   product_dispatch<Half, true>(op);
 }
 
-extern "C" __global__ void __launch_bounds__(kThreads, 1)
+extern "C" __global__ void __launch_bounds__(kPlainThreads, 1)
 ctb_qgemm_i8_stream(const signed char* x, const signed char* w, const float* x_scale, const float* w_scale,
                     const __half* bias, __half* output, int m, int n, int k, CTB_RESERVED_PARAMS) {
   (void)profile_scratch;
@@ -321,7 +332,7 @@ ctb_qgemm_i8_stream(const signed char* x, const signed char* w, const float* x_s
   product_dispatch<Int8, false>(op);
 }
 
-extern "C" __global__ void __launch_bounds__(kThreads, 1)
+extern "C" __global__ void __launch_bounds__(kGatedThreads, 1)
 ctb_qgated_gemm_i8_stream(const signed char* x, const signed char* w_gate, const signed char* w_up,
                           const float* x_scale, const float* gate_scale, const float* up_scale, __half* output, int m,
                           int n, int k, int activation, CTB_RESERVED_PARAMS) {

@@ -615,7 +615,7 @@ def _product_specs() -> list[KernelSpec]:
                               **pair))))
         # Few rows, weights by output channel: chosen at run time, as M is what
         # shape profiles leave open.
-        stream = dict(num_warps=20, shared_memory_bytes=231424, programmatic_launch=True)
+        stream = dict(num_warps=16 if gated else 20, shared_memory_bytes=231424, programmatic_launch=True)
         few_rows = {"kind": "dim_le", "source": "input", "index": 0, "axis": 0, "value": 16, "at_run": 1}
         stream_turned = {a.name: {"prepack": "transpose_2d"} for a in matrices}
         specs.append(KernelSpec(

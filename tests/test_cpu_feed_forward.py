@@ -204,7 +204,10 @@ def test_launch_shapes_match_the_kernels():
                 need = constant(spec.source, "kRingBytes") + 16 * 32 * 32 * 2 + 200 + 1024
                 assert need <= variant.shared_memory_bytes <= 232448
             elif spec.source == "product_stream.cu":
-                assert variant.num_warps == constant(spec.source, "kWarps") + constant(spec.source, "kJoinWarps")
+                readers = 16 if spec.op_type == "QGemm" else 12
+                name = "kPlainThreads" if spec.op_type == "QGemm" else "kGatedThreads"
+                assert f"constexpr int {name} = ({readers} + kJoinWarps) * 32;" in (folder / spec.source).read_text()
+                assert variant.num_warps == readers + constant(spec.source, "kJoinWarps")
                 assert variant.shared_memory_bytes == constant(spec.source, "kSharedBytes") <= 232448
             elif spec.source == "quantize.cu":
                 warps = constant(spec.source, "kWarps")
