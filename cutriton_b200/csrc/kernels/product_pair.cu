@@ -138,10 +138,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 // Without release: what the CTAs tell each other here are barrier
 // initialisations (fenced by mbar_init_fence) and that they have ended; a
 // releasing arrival waits for the epilogue's stores, 0.5 us and more.
-__device__ __forceinline__ void cluster_sync() {
+__device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ uint32_t cluster_addr(const void* local, uint32_t rank) {
   uint32_t remote;
@@ -308,10 +308,84 @@ __device__ __forceinline__ void finish(const Operands& op, uint32_t (&v)[kChunk]
   }
 }
 
+__device__ __forceinline__ Barriers* barriers(uint8_t* smem) {
+  return reinterpret_cast<Barriers*>(smem + kRingBytes + kStagingBytes);
+}
+
+// Publishes warp 1's TMEM allocation to the issuer and the epilogue warps.
+__device__ __forceinline__ uint32_t tmem_address(Barriers* bars) {
+  tc_fence_before_sync();
+  asm volatile("bar.sync 1, %0;" ::"n"(kThreads - 32) : "memory");
+  tc_fence_after_sync();
+  return *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
+}
+
+// The MMAs of all tiles, by warp 1 of the pair's leader.
+template <typename T>
+__device__ __forceinline__ void issue_mmas(uint8_t* smem, Barriers* bars, const Shape& sh, uint32_t tmem, int tiles,
+                                           int pair, int pairs, int k_blocks, void* scratch) {
+  volatile int* abort = &bars->abort;
+  const int stage_bytes = sh.blocks * sh.block_bytes;
+  // The whole warp runs the loop and one lane issues, so that descriptors
+  // are uniform values: by a lone thread four MMAs and two commits took 570
+  // clocks a stage, more than the 512 that the tensor cores need for it.
+  const uint32_t idesc = T::idesc(2 * kBM, 2 * sh.half);
+  const uint64_t a_first = smem_desc_kmajor_sw128(smem);
+  const uint64_t b_first = smem_desc_kmajor_sw128(smem + sh.x_bytes);
+  const uint32_t empty_first = smem_addr(&bars->empty[0]);
+  int s = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int tile = pair, local = 0; tile < tiles && ok; tile += pairs, ++local) {
+    const int buf = local & 1;
+    if (local >= 2 && !warp_wait(&bars->tmem_empty[buf], ((local >> 1) - 1) & 1, abort, scratch, 72)) {
+      ok = false;
+      break;
+    }
+    tc_fence_after_sync();
+    const uint32_t acc = tmem + buf * 256;
+    for (int kb = 0; kb < k_blocks; kb += sh.blocks) {
+      if (!warp_wait(&bars->full[s], phase, abort, scratch, 73)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after_sync();
+      if (elect_one()) {
+        const int blocks = min(sh.blocks, k_blocks - kb);
+        uint32_t offset = static_cast<uint32_t>(s * stage_bytes) >> 4;
+        for (int b = 0; b < blocks; ++b, offset += static_cast<uint32_t>(sh.block_bytes) >> 4) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            umma_pair(T{}, acc, a_first + offset + 2 * kk, b_first + offset + 2 * kk, idesc, (kb | b | kk) != 0);
+          }
+        }
+        umma_commit_pair(empty_first + 8 * s);
+      }
+      __syncwarp();
+      if (++s == sh.stages) {
+        s = 0;
+        phase ^= 1;
+      }
+    }
+    if (ok && elect_one()) umma_commit_pair(smem_addr(&bars->tmem_full[buf]));
+    __syncwarp();
+  }
+  if (!ok) {
+    if (elect_one()) {
+      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                       smem_addr(&bars->drain))
+                   : "memory");
+    }
+    volatile int never = 0;
+    mbar_wait(&bars->drain, 0, &never, scratch, 74);
+    __syncwarp();
+  }
+}
+
 template <typename T, bool kGated>
 __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, const Shape sh) {
   uint8_t* staging = smem + kRingBytes;
-  Barriers* bars = reinterpret_cast<Barriers*>(staging + kStagingBytes);
+  Barriers* bars = barriers(smem);
   volatile int* abort = &bars->abort;
   const int stage_bytes = sh.blocks * sh.block_bytes;
 
@@ -325,33 +399,6 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
   const int tiles = sh.m_tiles * sh.n_tiles;
   const bool tma_epilogue = op.n % 8 == 0 && ctb::aligned16(op.out);
   const TmaDescriptor* my_w = kGated && !leader ? op.w[1] : op.w[0];
-
-  if (warp == 0) {
-    for (int i = lane; i < 2 * kMaxStages; i += 32) mbar_init(&bars->full[0] + i, 1);  // full, then empty
-    if (lane < 2) mbar_init(&bars->tmem_full[lane], 1);
-    if (lane < 2) mbar_init(&bars->tmem_empty[lane], 2 * 4 * sh.active);
-    if (lane == 2) mbar_init(&bars->drain, 1);
-    if (lane == 3) bars->abort = 0;
-    mbar_init_fence();
-  } else if (warp == 1 && lane == 0) {
-    tma_prefetch(op.x);
-    tma_prefetch(my_w);
-    if (tma_epilogue) tma_prefetch(op.out_map);
-  }
-  // The peer's copies and commits reach these barriers: both CTAs have
-  // initialised them before either goes on.
-  cluster_sync();
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&bars->tmem_base)),
-                 "r"(kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = bars->tmem_base;
-  CTB_GRID_DEPENDENCY_SYNC();
 
   if (warp == 0) {
     // ---- TMA producer: this CTA's rows of x and of the weights ----
@@ -403,67 +450,27 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
       }
     }
     __syncwarp();
-  } else if (warp == 1 && leader) {
-    // ---- MMA issuer (pair leader) ----
-    // The whole warp runs the loop and one lane issues, so that descriptors
-    // are uniform values: by a lone thread four MMAs and two commits took 570
-    // clocks a stage, more than the 512 that the tensor cores need for it.
-    const uint32_t idesc = T::idesc(2 * kBM, 2 * sh.half);
-    const uint64_t a_first = smem_desc_kmajor_sw128(smem);
-    const uint64_t b_first = smem_desc_kmajor_sw128(smem + sh.x_bytes);
-    const uint32_t empty_first = smem_addr(&bars->empty[0]);
-    int s = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int tile = pair, local = 0; tile < tiles && ok; tile += pairs, ++local) {
-      const int buf = local & 1;
-      if (local >= 2 && !warp_wait(&bars->tmem_empty[buf], ((local >> 1) - 1) & 1, abort, op.scratch, 72)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after_sync();
-      const uint32_t acc = tmem + buf * 256;
-      for (int kb = 0; kb < k_blocks; kb += sh.blocks) {
-        if (!warp_wait(&bars->full[s], phase, abort, op.scratch, 73)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after_sync();
-        if (elect_one()) {
-          const int blocks = min(sh.blocks, k_blocks - kb);
-          uint32_t offset = static_cast<uint32_t>(s * stage_bytes) >> 4;
-          for (int b = 0; b < blocks; ++b, offset += static_cast<uint32_t>(sh.block_bytes) >> 4) {
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              umma_pair(T{}, acc, a_first + offset + 2 * kk, b_first + offset + 2 * kk, idesc, (kb | b | kk) != 0);
-            }
-          }
-          umma_commit_pair(empty_first + 8 * s);
-        }
-        __syncwarp();
-        if (++s == sh.stages) {
-          s = 0;
-          phase ^= 1;
-        }
-      }
-      if (ok && elect_one()) umma_commit_pair(smem_addr(&bars->tmem_full[buf]));
-      __syncwarp();
+  } else if (warp == 1) {
+    // ---- TMEM, and the MMA issuer (pair leader) ----
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&bars->tmem_base)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    if (leader) {
+      if (lane < 2) mbar_init(&bars->tmem_empty[lane], 2 * 4 * sh.active);
+      mbar_init_fence();
     }
-    if (!ok) {
-      if (elect_one()) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                       smem_addr(&bars->drain))
-                   : "memory");
-      volatile int never = 0;
-      mbar_wait(&bars->drain, 0, &never, op.scratch, 74);
-      __syncwarp();
-    }
-  } else if (warp >= kEpilogueWarp0 && (warp - kEpilogueWarp0) / 4 < sh.active) {
+    const uint32_t tmem = tmem_address(bars);
+    if (leader) issue_mmas<T>(smem, bars, sh, tmem, tiles, pair, pairs, k_blocks, op.scratch);
+  } else {
     // ---- epilogue: this CTA's 128 rows, quarter = warp % 4 ----
+    const uint32_t tmem = tmem_address(bars);
     const int quarter = warp & 3;
     const int wq = (warp - kEpilogueWarp0) / 4;
     uint8_t* box_smem = staging + (warp - kEpilogueWarp0) * kStageBoxBytes;
     bool box_used = false;
-    for (int tile = pair, local = 0; tile < tiles; tile += pairs, ++local) {
+    // (Warps without a chunk take no part.)
+    for (int tile = wq < sh.active ? pair : tiles, local = 0; tile < tiles; tile += pairs, ++local) {
       const int buf = local & 1;
       int mt, nt;
       tile_at(tile, sh, &mt, &nt);
@@ -540,10 +547,11 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
   tc_fence_before_sync();
   __syncthreads();
   // Neither CTA leaves (or frees TMEM) while its peer may still signal it.
-  cluster_sync();
+  cluster_arrive();
+  cluster_wait();
   tc_fence_after_sync();
-  if (warp == 0) {
-    __syncwarp();
+  if (warp == 1) {
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
 }
@@ -587,6 +595,18 @@ __device__ __forceinline__ void product_dispatch(Operands& op, const TmaDescript
                                                  const Boxes& w0, const Boxes& w1) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+  if (threadIdx.x < 32) {
+    Barriers* bars = barriers(smem);
+    const int lane = threadIdx.x;
+    if (lane < 2 * kMaxStages) mbar_init(&bars->full[0] + lane, 1);  // full, then empty
+    if (lane < 2) mbar_init(&bars->tmem_full[lane], 1);
+    if (lane == 2) mbar_init(&bars->drain, 1);
+    if (lane == 3) bars->abort = 0;
+    mbar_init_fence();
+  }
+  // The peer's copies and commits reach these barriers: both CTAs have
+  // initialised them before either goes on. The shape is computed meanwhile.
+  cluster_arrive();
   const Shape sh = shape_of<kGated>(choose_width<kGated>(op.m, op.n, gridDim.x / 2), op.m, op.n);
   op.x = sh.x_box == 0 ? x[0] : sh.x_box == 1 ? x[1] : x[2];
   const auto pick = [&](const Boxes& w) {
@@ -594,6 +614,8 @@ __device__ __forceinline__ void product_dispatch(Operands& op, const TmaDescript
   };
   op.w[0] = pick(w0);
   op.w[1] = kGated ? pick(w1) : nullptr;
+  cluster_wait();
+  CTB_GRID_DEPENDENCY_SYNC();
   product_pair<T, kGated>(smem, op, sh);
 }
 
