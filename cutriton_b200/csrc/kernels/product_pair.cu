@@ -72,6 +72,9 @@ constexpr int kHalves = 5;
 constexpr int kXBoxes = 3;
 __device__ __forceinline__ int half_at(int i) { return i == 0 ? 128 : i == 1 ? 96 : i == 2 ? 64 : i == 3 ? 48 : 32; }
 __device__ __forceinline__ int x_rows_at(int i) { return 128 >> i; }
+// 64 or 32 rows a CTA where the pair's two hold all of M: a block of 128 rows
+// takes 250 clocks through TMA, as long as the rest of a block's round.
+__device__ __forceinline__ int x_box_for(int m) { return m > 128 ? 0 : m > 64 ? 1 : 2; }
 
 // a / b for 0 <= a, 0 < b with 1 / b at hand: an integer division by a value
 // known at run time only takes some 150 clocks of a kernel's start.
@@ -87,7 +90,8 @@ struct Shape {
   int width;             // index of half
   int half;              // weight rows a CTA
   int columns;           // output columns
-  int x_box;             // index of the box of x: the least that holds min(M, 128) rows
+  int x_box;             // index of the box of x
+  int rows;              // of x a CTA, the box's: the pair shares up to 64 or 128 rows out evenly
   int x_bytes, block_bytes;  // of a block of K: rows of x, and with the weight rows
   int blocks;            // of K a stage
   int stages;
@@ -102,8 +106,9 @@ __device__ __forceinline__ Shape shape_of(int width, int m, int n) {
   s.width = width;
   s.half = half_at(width);
   s.columns = kGated ? s.half : 2 * s.half;
-  s.x_box = m > 64 ? 0 : m > 32 ? 1 : 2;
-  s.x_bytes = x_rows_at(s.x_box) * kRowBytes;
+  s.x_box = x_box_for(m);
+  s.rows = x_rows_at(s.x_box);
+  s.x_bytes = s.rows * kRowBytes;
   s.block_bytes = s.x_bytes + s.half * kRowBytes;  // a multiple of 1024
   // Short blocks share a stage, one round of barriers for two or four of them
   // (32x12288x4096 in 8 bits: one 21.7, two 18.7, four 15.6 us), as long as
@@ -112,7 +117,7 @@ __device__ __forceinline__ Shape shape_of(int width, int m, int n) {
   const int ring_blocks = static_cast<int>(kRingBytes / static_cast<float>(s.block_bytes));
   s.blocks = ring_blocks >= 20 ? 4 : ring_blocks >= 8 ? 2 : 1;
   s.stages = min(kMaxStages, s.blocks == 4 ? ring_blocks / 4 : s.blocks == 2 ? ring_blocks / 2 : ring_blocks);
-  s.m_tiles = (m + 2 * kBM - 1) / (2 * kBM);
+  s.m_tiles = (m + 2 * s.rows - 1) / (2 * s.rows);  // by a power of two
   s.n_tiles = quotient(n + s.columns - 1, s.columns, __frcp_rn(static_cast<float>(s.columns)));
   s.chunks = (s.columns + kChunk - 1) / kChunk;
   s.active = min(s.chunks, kEpilogueWarps / 4);
@@ -409,13 +414,13 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
     for (int tile = pair; tile < tiles && ok; tile += pairs) {
       int mt, nt;
       tile_at(tile, sh, &mt, &nt);
-      const int pair_m0 = mt * 2 * kBM;
-      const int m0 = pair_m0 + static_cast<int>(rank) * kBM;
+      const int pair_m0 = mt * 2 * sh.rows;
+      const int m0 = pair_m0 + static_cast<int>(rank) * sh.rows;
       const int n0 = nt * sh.columns + (kGated ? 0 : static_cast<int>(rank) * sh.half);
       // Rows of x past M keep what the stage held: their sums are not stored,
       // and a CTA without rows loads none.
       const bool has_x = m0 < op.m;
-      const int pair_bytes = 2 * sh.half * kRowBytes + (pair_m0 + kBM < op.m ? 2 : 1) * sh.x_bytes;
+      const int pair_bytes = 2 * sh.half * kRowBytes + (pair_m0 + sh.rows < op.m ? 2 : 1) * sh.x_bytes;
       for (int kb = 0; kb < k_blocks; kb += sh.blocks) {
         if (!warp_wait(&bars->empty[s], phase, abort, op.scratch, 70)) {
           ok = false;
@@ -474,9 +479,10 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
       const int buf = local & 1;
       int mt, nt;
       tile_at(tile, sh, &mt, &nt);
-      const int row0 = mt * 2 * kBM + static_cast<int>(rank) * kBM + quarter * 32;
+      const int row0 = (2 * mt + static_cast<int>(rank)) * sh.rows + quarter * 32;
+      const bool has_rows = quarter * 32 < sh.rows && row0 < op.m;
       const int n0 = nt * sh.columns;
-      const float row_scale = op.x_scale != nullptr && row0 + lane < op.m ? __ldg(op.x_scale + row0 + lane) : 0.0f;
+      const float row_scale = op.x_scale != nullptr && has_rows && row0 + lane < op.m ? __ldg(op.x_scale + row0 + lane) : 0.0f;
       const bool ready = mbar_wait(&bars->tmem_full[buf], (local >> 1) & 1, abort, op.scratch, 75);
       __syncwarp();
       if (!ready) break;
@@ -504,7 +510,7 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
           }
         }
         // Columns past N (a partial last tile) and rows past M: nothing to store.
-        if (n0 + c >= op.n || row0 >= op.m) continue;
+        if (n0 + c >= op.n || !has_rows) continue;
         uint4 packed[kChunk / 8];
         finish<T, kGated>(op, v, u, n0 + c, row_scale, packed);
         if (box_used) {
@@ -575,7 +581,7 @@ __device__ __forceinline__ int choose_width(int m, int n, int pairs) {
   const float columns = kGated ? half : 2.0f * half;
   const float m_tiles = static_cast<float>((m + 2 * kBM - 1) / (2 * kBM));
   const float tiles = m_tiles * ceilf(__fdividef(static_cast<float>(n), columns));
-  const float x_rows = m > 64 ? 128.0f : m > 32 ? 64.0f : 32.0f;
+  const float x_rows = static_cast<float>(x_rows_at(x_box_for(m)));
   const float busy = fmaxf(4.0f * half + 52.0f, 268.0f + 0.85f * x_rows);
   const float hbm = __fdividef(5.6f * half, m_tiles);
   const float waves = __fdividef(tiles, static_cast<float>(pairs));
