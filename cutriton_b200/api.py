@@ -157,7 +157,7 @@ def _to_model(ir: dict[str, Any], shapes: dict[str, tuple[int, ...]], dtypes: di
             out = {"transB": int(attrs.get("transB", 0))}
             if op != "QGemm":
                 activation = attrs.get("activation", "silu")
-                if activation not in _ACTIVATIONS and activation not in _ACTIVATIONS.values():
+                if not isinstance(activation, (str, int)) or activation not in {**_ACTIVATIONS, 0: 0, 1: 1}:
                     raise UnsupportedModelError(f"{where}: activation must be 'silu' or 'gelu'")
                 out["activation"] = _ACTIVATIONS.get(activation, activation)
         else:

@@ -368,12 +368,13 @@ class CudaSm100Backend final : public Backend {
       steps.push_back({"Gemm", in, {projected}});
       steps.push_back({"Gelu", {projected}, {out}});
     } else if (op == "GatedGemm") {
+      // The gate's slot serves the up projection once it is activated.
       const std::string gate = temp("gate", 0);
-      const std::string up = temp("up", 1);
-      const std::string activated = temp("activated", 2);
+      const std::string activated = temp("activated", 1);
+      const std::string up = temp("up", 0);
       steps.push_back({"Gemm", {in[0], in[1]}, {gate}});
-      steps.push_back({"Gemm", {in[0], in[2]}, {up}});
       steps.push_back({GetIntAttribute(node, "activation", 0) == 0 ? "Silu" : "Gelu", {gate}, {activated}});
+      steps.push_back({"Gemm", {in[0], in[2]}, {up}});
       steps.push_back({"Mul", {activated, up}, {out}});
     } else if (op == "SkipLayerNormalization") {
       const std::string sum = temp("add", 0);

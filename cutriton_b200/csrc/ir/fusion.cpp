@@ -46,7 +46,7 @@ Status RegisterBuiltinFusionAlternatives() {
        {"FusedConvBatchNorm", "AddRelu"}},
       {"AddRelu", "unfused:add_relu", {"Add", "Relu"}},
       {"GemmGelu", "unfused:gemm_gelu", {"Gemm", "Gelu"}},
-      {"GatedGemm", "unfused:gated_gemm", {"Gemm", "Gemm", "Silu", "Mul"}},
+      {"GatedGemm", "unfused:gated_gemm", {"Gemm", "Silu", "Gemm", "Mul"}},
       {"SkipLayerNormalization", "unfused:add_layer_norm", {"Add", "LayerNormalization"}},
   };
   auto& registry = FusionRegistry::Global();

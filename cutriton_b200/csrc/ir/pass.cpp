@@ -527,6 +527,13 @@ class GatedGemmFusionPass final : public GraphPass {
         if (!half_gemm(gate) || !half_gemm(up) || gate == up || gate->inputs()[0] != up->inputs()[0]) continue;
         const int64_t tb = GetIntAttribute(*gate, "transB", 0);
         if (tb != GetIntAttribute(*up, "transB", 0)) continue;
+        // [K, N] weights are turned at upload; ones that are computed or bound
+        // stay with the Gemm kernels, which read them as they are.
+        const auto constant = [&](const std::string& name) {
+          const ValueDesc* v = g->FindValue(name);
+          return v != nullptr && v->is_constant;
+        };
+        if (tb == 0 && (!constant(gate->inputs()[1]) || !constant(up->inputs()[1]))) continue;
         const int64_t activation = act->op_type() == "Silu" ? 0 : 1;
         std::vector<std::string> inputs = {gate->inputs()[0], gate->inputs()[1], up->inputs()[1]};
         *removed = {gate->id(), act->id(), up->id()};

@@ -76,13 +76,23 @@ __device__ __forceinline__ int x_rows_at(int i) { return 128 >> i; }
 // takes 250 clocks through TMA, as long as the rest of a block's round.
 __device__ __forceinline__ int x_box_for(int m) { return m > 128 ? 0 : m > 64 ? 1 : 2; }
 
-// a / b for 0 <= a, 0 < b with 1 / b at hand: an integer division by a value
-// known at run time only takes some 150 clocks of a kernel's start.
-__device__ __forceinline__ int quotient(int a, int b, float inverse) {
-  int q = static_cast<int>(static_cast<float>(a) * inverse);
-  while (static_cast<long long>(q) * b > a) --q;
-  while (static_cast<long long>(q + 1) * b <= a) ++q;
+// a / b for 0 <= a, 0 < b: the FP32 quotient is off by a few units at most
+// and set right by the remainder. (An integer division by a value known at run
+// time only takes some 150 clocks of a kernel's start.)
+__device__ __forceinline__ int quotient(int a, int b) {
+  int q = static_cast<int>(static_cast<float>(a) * ctb::reciprocal(static_cast<float>(b)));
+  int r = a - q * b;
+  for (; r < 0; r += b) --q;
+  for (; r >= b; r -= b) ++q;
   return q;
+}
+
+// Tiles of 2^shift or 3 * 2^shift columns over n: half is 128, 64, 32 or 96, 48.
+__device__ __forceinline__ int column_tiles(int n, int columns) {
+  const bool three = columns % 3 == 0;  // (a compile-time divisor)
+  const int shift = three ? 31 - __clz(columns / 3) : 31 - __clz(columns);
+  const unsigned t = static_cast<unsigned>(n + columns - 1) >> shift;
+  return static_cast<int>(three ? t / 3u : t);
 }
 
 // A tile's width and what follows from it.
@@ -114,11 +124,12 @@ __device__ __forceinline__ Shape shape_of(int width, int m, int n) {
   // (32x12288x4096 in 8 bits: one 21.7, two 18.7, four 15.6 us), as long as
   // enough stages are left (with three of two blocks 256x4096x12288 took 58
   // instead of 51 us).
-  const int ring_blocks = static_cast<int>(kRingBytes / static_cast<float>(s.block_bytes));
+  const int ring_blocks =
+      static_cast<int>(kRingBytes * ctb::reciprocal(static_cast<float>(s.block_bytes)) + 1e-3f);  // 6 to 24
   s.blocks = ring_blocks >= 20 ? 4 : ring_blocks >= 8 ? 2 : 1;
   s.stages = min(kMaxStages, s.blocks == 4 ? ring_blocks / 4 : s.blocks == 2 ? ring_blocks / 2 : ring_blocks);
-  s.m_tiles = (m + 2 * s.rows - 1) / (2 * s.rows);  // by a power of two
-  s.n_tiles = quotient(n + s.columns - 1, s.columns, __frcp_rn(static_cast<float>(s.columns)));
+  s.m_tiles = (m + 2 * s.rows - 1) >> (8 - s.x_box);
+  s.n_tiles = column_tiles(n, s.columns);
   s.chunks = (s.columns + kChunk - 1) / kChunk;
   s.active = min(s.chunks, kEpilogueWarps / 4);
   return s;
@@ -260,12 +271,12 @@ __device__ __forceinline__ void tile_at(int index, const Shape& sh, int* mt, int
   int first = 0;  // tile row
   if (sh.m_tiles > kRasterRows) {
     const int per_block = kRasterRows * sh.n_tiles;
-    const int block = quotient(index, per_block, __frcp_rn(static_cast<float>(per_block)));
+    const int block = quotient(index, per_block);
     index -= block * per_block;
     first = block * kRasterRows;
   }
   const int rows = min(kRasterRows, sh.m_tiles - first);
-  *nt = rows == 1 ? index : quotient(index, rows, __frcp_rn(static_cast<float>(rows)));
+  *nt = rows == 1 ? index : quotient(index, rows);
   *mt = first + index - *nt * rows;
 }
 
@@ -302,7 +313,7 @@ __device__ __forceinline__ void finish(const Operands& op, uint32_t (&v)[kChunk]
       for (int j = 0; j < kChunk; ++j) y[j] = ctb::silu_fast(y[j]) * __uint_as_float(u[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < kChunk; ++j) y[j] = ctb::gelu_erf_fast(y[j]) * __uint_as_float(u[j]);
+      for (int j = 0; j < kChunk; ++j) y[j] = ctb::gelu_fast(y[j]) * __uint_as_float(u[j]);
     }
   }
 #pragma unroll
@@ -513,6 +524,18 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
         if (n0 + c >= op.n || !has_rows) continue;
         uint4 packed[kChunk / 8];
         finish<T, kGated>(op, v, u, n0 + c, row_scale, packed);
+        const int end = min(op.n, n0 + sh.columns);
+        if (tma_epilogue && c + kChunk > sh.columns) {
+          // Half a chunk (gated, half = 48): each lane its row's 32 bytes.
+          if (row0 + lane < op.m) {
+            __half* dst = op.out + static_cast<long long>(row0 + lane) * op.n + n0 + c;
+#pragma unroll
+            for (int i = 0; i < kChunk / 16; ++i) {
+              if (n0 + c + 8 * i < end) *reinterpret_cast<uint4*>(dst + 8 * i) = packed[i];
+            }
+          }
+          continue;
+        }
         if (box_used) {
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
@@ -522,7 +545,7 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
         for (int i = 0; i < kChunk / 8; ++i) {
           *reinterpret_cast<uint4*>(box_smem + lane * 64 + (((i ^ (lane >> 1)) & 3) << 4)) = packed[i];
         }
-        if (tma_epilogue && c + kChunk <= sh.columns) {
+        if (tma_epilogue) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
@@ -532,18 +555,25 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
           box_used = true;
         } else {
           // Rows that TMA cannot address (N no multiple of 8, an output off
-          // 16 bytes) and half chunks: one row of the chunk a store instruction.
+          // 16 bytes): one row of the chunk a store instruction, eight under way.
           __syncwarp();
           const int column = n0 + c + lane;
-          const int end = min(op.n, n0 + sh.columns);
-#pragma unroll 4
-          for (int r = 0; r < 32 && row0 + r < op.m; ++r) {
-            const __half h = *reinterpret_cast<const __half*>(
-                box_smem + r * 64 + ((((lane >> 3) ^ (r >> 1)) & 3) << 4) + (lane & 7) * 2);
-            if (column < end) op.out[static_cast<long long>(row0 + r) * op.n + column] = h;
+          const int rows = column < end ? op.m - row0 : 0;
+          __half* dst = op.out + static_cast<long long>(row0) * op.n + column;
+#pragma unroll
+          for (int r0 = 0; r0 < 32; r0 += 8) {
+            __half h[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+              h[r] = *reinterpret_cast<const __half*>(
+                  box_smem + (r0 + r) * 64 + ((((lane >> 3) ^ ((r0 + r) >> 1)) & 3) << 4) + (lane & 7) * 2);
+            }
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+              if (r0 + r < rows) dst[static_cast<long long>(r0 + r) * op.n] = h[r];
+            }
           }
           __syncwarp();
-          box_used = false;
         }
       }
     }
@@ -578,13 +608,11 @@ __device__ __forceinline__ int choose_width(int m, int n, int pairs) {
   const int lane = threadIdx.x & 31;
   const int width = min(lane, kHalves - 1);
   const float half = static_cast<float>(half_at(width));
-  const float columns = kGated ? half : 2.0f * half;
-  const float m_tiles = static_cast<float>((m + 2 * kBM - 1) / (2 * kBM));
-  const float tiles = m_tiles * ceilf(__fdividef(static_cast<float>(n), columns));
-  const float x_rows = static_cast<float>(x_rows_at(x_box_for(m)));
-  const float busy = fmaxf(4.0f * half + 52.0f, 268.0f + 0.85f * x_rows);
-  const float hbm = __fdividef(5.6f * half, m_tiles);
-  const float waves = __fdividef(tiles, static_cast<float>(pairs));
+  const int m_tiles = (m + 2 * kBM - 1) / (2 * kBM);
+  const float tiles = static_cast<float>(m_tiles) * static_cast<float>(column_tiles(n, half_at(width) * (kGated ? 1 : 2)));
+  const float busy = fmaxf(4.0f * half + 52.0f, 268.0f + 0.85f * static_cast<float>(x_rows_at(x_box_for(m))));
+  const float hbm = 5.6f * half * ctb::reciprocal(static_cast<float>(m_tiles));
+  const float waves = tiles * ctb::reciprocal(static_cast<float>(pairs));
   const float full = floorf(waves + 1e-3f);
   const float rest = fmaxf(0.0f, waves - full);
   float clocks = full * fmaxf(busy, hbm) + (rest > 1e-3f ? fmaxf(busy, hbm * rest) : 0.0f);

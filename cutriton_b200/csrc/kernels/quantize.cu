@@ -68,10 +68,10 @@ __device__ __noinline__ uint2 quantize_settled(uint4 v, float s, float inv) {
   return make_uint2(low_bytes(t[0], t[1], t[2], t[3]), low_bytes(t[4], t[5], t[6], t[7]));
 }
 
-// Eight integers of one vector, a byte each. inv is 1 / s to 2^-22: |x inv|
-// is at most 127.1, so a quotient is off by less than 2^-15 + 2^-17 and where
-// its roundings with an inverse 2^-21 smaller and larger agree (the tests'
-// 2^-21 of 127 is 2^-14), the exact one does too. Else it is settled exactly.
+// Eight integers of one vector, a byte each. inv is 1 / s to 2^-23, so the
+// quotient lies between x (1 - 2^-21) inv and x (1 + 2^-21) inv, and where
+// those two round to the same integer (they are 2^-13 apart at most), so does
+// it. Else, about once in 10^4 elements, it is settled exactly.
 __device__ __forceinline__ uint2 quantize(uint4 v, float s, float inv) {
   const __half2* h = reinterpret_cast<const __half2*>(&v);
   const float below = inv * (1.0f - 0x1p-21f), above = inv * (1.0f + 0x1p-21f);

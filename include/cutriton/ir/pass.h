@@ -39,7 +39,8 @@ std::unique_ptr<GraphPass> CreateConvBatchNormReluFusionPass();
 // Add -> Relu  =>  AddRelu.
 std::unique_ptr<GraphPass> CreateAddReluFusionPass();
 // Gemm -> Silu | Gelu, Mul with a second float16 Gemm of the same input  =>
-// GatedGemm (every value between single-consumer and no graph output).
+// GatedGemm (every value between single-consumer and no graph output; weights
+// constant, or by rows with transB).
 // sm_100a extension, part of the transformer fusions.
 std::unique_ptr<GraphPass> CreateGatedGemmFusionPass();
 // Gemm -> Gelu  =>  GemmGelu (Gemm output single-consumer, not a graph output).

@@ -136,6 +136,26 @@ def test_chain_whose_values_are_used_elsewhere_stays(kwargs):
     assert "GatedGemm" not in [op["op_type"] for op in engine.ops()]
 
 
+@pytest.mark.parametrize("trans_b,fused", [(0, False), (1, True)])
+def test_weights_that_are_graph_inputs_fuse_by_rows_only(trans_b, fused):
+    model = ct.Model()
+    model.add_input("x", [6, 32], dtype=np.float16, layout="")
+    for name in ("wg", "wu"):
+        model.add_input(name, [24, 32] if trans_b else [32, 24], dtype=np.float16, layout="")
+    model.add_node("gate", "Gemm", ["x", "wg"], ["g"], transB=trans_b)
+    model.add_node("act", "Silu", ["g"], ["a"])
+    model.add_node("up", "Gemm", ["x", "wu"], ["u"], transB=trans_b)
+    model.add_node("product", "Mul", ["a", "u"], ["y"])
+    model.add_output("y")
+    ops = [o["op_type"] for o in ct.build_engine(model).ops()]
+    assert ops == (["GatedGemm"] if fused else ["Gemm", "Silu", "Gemm", "Mul"])
+
+
+def test_unfused_candidate_needs_two_buffers():
+    """Gate and up projection share a slot: 2 x 6 x 24 FP16 in 256-byte slots."""
+    assert ct.build_engine(gated_chain()).workspace_bytes() == 2 * 512
+
+
 def test_transformer_fusions_off_keeps_the_chain():
     engine = ct.build_engine(gated_chain(), enable_transformer_fusions=0)
     assert [op["op_type"] for op in engine.ops()] == ["Gemm", "Silu", "Gemm", "Mul"]
@@ -237,7 +257,7 @@ def test_quantized_weight_holds_its_values():
     assert (error <= scale[:, None] * (0.5 + 128 * 2.0**-24)).all()
 
 
-@pytest.mark.parametrize("activation", ["silu", "gelu", 0, 1])
+@pytest.mark.parametrize("activation", ["silu", "gelu", 0, 1], ids=str)
 def test_facade_takes_the_operators(tmp_path, activation):
     import json
 
@@ -263,11 +283,13 @@ def test_facade_refuses_other_activations(tmp_path):
 
     graph = {"inputs": ["x", "a", "b"], "outputs": ["y"], "input_dtypes": {n: "float16" for n in "xab"},
              "nodes": [{"name": "g", "op_type": "GatedGemm", "inputs": ["x", "a", "b"], "outputs": ["y"],
-                        "activation": "tanh"}]}
+                        "activation": None}]}
     path = tmp_path / "g.json"
-    path.write_text(json.dumps(graph))
-    with pytest.raises(api.UnsupportedModelError):
-        api.compile(path).native({"x": (3, 16), "a": (16, 8), "b": (16, 8)})
+    for activation in ("tanh", 2, [0]):
+        graph["nodes"][0]["activation"] = activation
+        path.write_text(json.dumps(graph))
+        with pytest.raises(api.UnsupportedModelError):
+            api.compile(path).native({"x": (3, 16), "a": (16, 8), "b": (16, 8)})
 
 
 def test_scale_without_a_reader_is_planned():

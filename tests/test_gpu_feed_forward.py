@@ -170,6 +170,35 @@ def test_large_values_and_non_finite_rows(cuda):
         assert np.isfinite(y[[0, *range(3, m)]]).all()
 
 
+@pytest.mark.parametrize("rows", [5, 150])
+@pytest.mark.parametrize("activation", [ff.SILU, ff.GELU])
+def test_non_finite_weights_stay_in_their_column(cuda, activation, rows):
+    """NaN or infinities in single output channels; gates far out on the side
+    where the activation vanishes, next to ordinary ones."""
+    inputs = ff.gated_case(np.random.default_rng(13), rows, 96, 76)
+    inputs["x"] = np.abs(inputs["x"]) + np.float16(0.5)
+    bad = {3: np.nan, 10: np.inf, 11: -np.inf, 40: np.nan, 73: np.nan}
+    inputs["w_gate"][20] = -60000
+    inputs["w_gate"][21] = 60000
+    inputs["w_gate"][75] = -1
+    clean = {n: a.copy() for n, a in inputs.items()}
+    for column, value in bad.items():
+        inputs["w_gate" if column < 40 else "w_up"][column, column % 7] = value
+    expected, tol = ff.gated_result(clean, activation)
+    runner = Runner(ff.product_graph("GatedGemm", inputs, activation=activation, transB=1), inputs)
+    runner.output("y", (rows, 76), np.float16)
+    good = np.setdiff1d(np.arange(76), list(bad))
+    for index, name in enumerate(runner.engine.op(0)["candidates"]):
+        try:
+            y = runner.run(index)["y"]
+        except ct.CutritonError as error:
+            assert error.code == ct.SHAPE_ERROR and "stream" in name
+            continue
+        inside = good[np.abs(expected[:, good]).max(axis=0) < 65000]
+        assert (np.abs(y[:, inside].astype(np.float64) - expected[:, inside]) <= tol[:, inside]).all(), name
+        assert inside.size >= 65 and not np.isfinite(y[:, [3, 40, 73]]).any(), name
+
+
 @pytest.mark.parametrize("activation", [ff.SILU, ff.GELU])
 def test_unfused_gated_gemm(cuda, activation):
     """The decomposition rounds gate, activation and up projection to FP16
