@@ -9,6 +9,8 @@
 #include "cutriton/ir/pass.h"
 
 #include <algorithm>
+#include <initializer_list>
+#include <limits>
 #include <unordered_set>
 
 #include "cutriton/ir/op_schema.h"
@@ -158,6 +160,16 @@ Status InferGemm(Graph* graph, const Node& node) {
 
 // ---- gated and 8-bit products ----------------------------------------------------
 
+// The kernels index rows and columns in 32 bits, up to the end of a last tile.
+Status CheckExtents(const Node& node, std::initializer_list<int64_t> extents) {
+  for (const int64_t extent : extents) {
+    if (extent > std::numeric_limits<int32_t>::max() - 1024) {
+      return Status::Unsupported(node.op_type() + ": dimensions must be below 2^31 - 1024");
+    }
+  }
+  return Status::OK();
+}
+
 // The weight `name` of a product over x's K columns: [K, N], or [N, K] with
 // transB. Gives N.
 Status CheckWeight(const Graph& graph, const Node& node, const std::string& name, int64_t k, DataType dtype,
@@ -205,6 +217,7 @@ Status InferGatedGemm(Graph* graph, const Node& node) {
   CUTRITON_RETURN_IF_ERROR(CheckWeight(*graph, node, node.inputs()[1], k, x->tensor.dtype, &n));
   CUTRITON_RETURN_IF_ERROR(CheckWeight(*graph, node, node.inputs()[2], k, x->tensor.dtype, &n_up));
   if (n != n_up) return Status::ShapeError("GatedGemm gate and up weights must have the same width");
+  CUTRITON_RETURN_IF_ERROR(CheckExtents(node, {x->tensor.shape[0], n, k}));
   TensorDesc out = Derived(x->tensor, {x->tensor.shape[0], n}, "");
   CUTRITON_RETURN_IF_ERROR(out.Validate());
   return graph->SetValueDesc(node.outputs()[0], std::move(out));
@@ -216,6 +229,7 @@ Status InferQuantizeRows(Graph* graph, const Node& node) {
   if (x == nullptr || x->tensor.shape.size() != 2 || x->tensor.dtype != DataType::kFloat16) {
     return Status::ShapeError("QuantizeRows expects a rank-2 float16 input");
   }
+  CUTRITON_RETURN_IF_ERROR(CheckExtents(node, {x->tensor.shape[0], x->tensor.shape[1]}));
   TensorDesc q = Derived(x->tensor, x->tensor.shape, "");
   q.dtype = DataType::kInt8;
   TensorDesc scale = Derived(x->tensor, {x->tensor.shape[0]}, "");
@@ -239,6 +253,7 @@ Status CheckQuantizedRows(const Graph& graph, const Node& node, int64_t* m, int6
 }
 
 Status SetProduct(Graph* graph, const Node& node, int64_t m, int64_t n) {
+  CUTRITON_RETURN_IF_ERROR(CheckExtents(node, {m, n}));
   TensorDesc out = Derived(graph->FindValue(node.inputs()[0])->tensor, {m, n}, "");
   out.dtype = DataType::kFloat16;
   CUTRITON_RETURN_IF_ERROR(out.Validate());

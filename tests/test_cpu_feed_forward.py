@@ -78,6 +78,35 @@ def test_refusals(op, inputs, attributes, code):
     assert error.value.code == code, error.value
 
 
+HUGE = 2**31 - 1024
+
+
+@pytest.mark.parametrize("op,shapes", [
+    ("GatedGemm", dict(x=("f2", (HUGE, 8)), w_gate=("f2", (24, 8)), w_up=("f2", (24, 8)))),
+    ("GatedGemm", dict(x=("f2", (4, 8)), w_gate=("f2", (HUGE, 8)), w_up=("f2", (HUGE, 8)))),
+    ("GatedGemm", dict(x=("f2", (4, HUGE)), w_gate=("f2", (24, HUGE)), w_up=("f2", (24, HUGE)))),
+    ("QGemm", dict(x=("i1", (HUGE, 8)), x_scale=("f4", (HUGE,)), w=("i1", (24, 8)), w_scale=("f4", (24,)))),
+    ("QGemm", dict(x=("i1", (4, 8)), x_scale=("f4", (4,)), w=("i1", (HUGE, 8)), w_scale=("f4", (HUGE,)))),
+    ("QuantizeRows", dict(x=("f2", (HUGE, 2)))),
+    ("QuantizeRows", dict(x=("f2", (2, HUGE)))),
+])
+def test_dimensions_whose_last_tile_passes_32_bits_are_refused(op, shapes):
+    def build(shapes):
+        model = ct.Model()
+        for name, (dtype, shape) in shapes.items():
+            model.add_input(name, list(shape), dtype=dtype, layout="")
+        outs = ["q", "s"] if op == "QuantizeRows" else ["y"]
+        model.add_node("node", op, list(shapes), outs, **({} if op == "QuantizeRows" else {"transB": 1}))
+        for name in outs:
+            model.add_output(name)
+        return ct.build_engine(model)
+
+    with pytest.raises(ct.CutritonError) as error:
+        build(shapes)
+    assert error.value.code == ct.UNSUPPORTED and "2^31 - 1024" in str(error.value)
+    build({n: (d, tuple(v - 1 if v == HUGE else v for v in s)) for n, (d, s) in shapes.items()})
+
+
 @pytest.mark.parametrize("op,inputs", [("QGemm", {n: QGEMM[n] for n in ("x", "x_scale", "w")}),
                                        ("QGatedGemm", {n: QGATED[n] for n in list(QGATED)[:5]}),
                                        ("GatedGemm", {n: GATED[n] for n in ("x", "w_gate")})])
