@@ -10,7 +10,8 @@
 // 64 x 64 tiles, 256 threads of 4 x 4 outputs, K in chunks of 32 through
 // shared memory; 8-bit operands lie there four k to a word (dp4a). FP32 and
 // integer units bound it, far below the tensor cores' rate; every access is
-// one element, so nothing has to be aligned.
+// one element, so nothing has to be aligned. The blocks of one column of tiles
+// are neighbours in a grid of one dimension (the second one ends at 65535).
 
 #include "product.cuh"
 
@@ -66,6 +67,13 @@ __device__ __forceinline__ void stage(typename T::Word (&words)[kChunk / T::kPer
   }
 }
 
+// First row and column of this block's tile.
+__device__ __forceinline__ void tile_origin(int m, long long* m0, long long* n0) {
+  const unsigned m_tiles = (static_cast<unsigned>(m) + kTile - 1) / kTile;
+  *m0 = static_cast<long long>(blockIdx.x % m_tiles) * kTile;
+  *n0 = static_cast<long long>(blockIdx.x / m_tiles) * kTile;
+}
+
 template <typename T, int kOperands>
 __device__ __forceinline__ void tile_sums(typename T::Sum (&sum)[kOperands][4][4],
                                           const typename T::Element* x, const typename T::Element* const (&w)[kOperands],
@@ -74,7 +82,8 @@ __device__ __forceinline__ void tile_sums(typename T::Sum (&sum)[kOperands][4][4
   __shared__ typename T::Word xs[kWords][kTile + 1];
   __shared__ typename T::Word ws[kOperands][kWords][kTile + 1];
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const long long m0 = static_cast<long long>(blockIdx.x) * kTile, n0 = static_cast<long long>(blockIdx.y) * kTile;
+  long long m0, n0;
+  tile_origin(m, &m0, &n0);
 #pragma unroll
   for (int o = 0; o < kOperands; ++o)
 #pragma unroll
@@ -108,12 +117,13 @@ __device__ __forceinline__ void tile_sums(typename T::Sum (&sum)[kOperands][4][4
 template <typename F>
 __device__ __forceinline__ void each_output(int m, int n, F store) {
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  long long m0, n0;
+  tile_origin(m, &m0, &n0);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const long long row = static_cast<long long>(blockIdx.x) * kTile + ty + 16 * i;
-      const long long column = static_cast<long long>(blockIdx.y) * kTile + tx + 16 * j;
+      const long long row = m0 + ty + 16 * i, column = n0 + tx + 16 * j;
       if (row < m && column < n) store(row, column, i, j);
     }
 }

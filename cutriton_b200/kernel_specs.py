@@ -582,7 +582,7 @@ def _product_specs() -> list[KernelSpec]:
             kernel_id=f"{name}.{tag}.any", op_type=op_type, version=1, source="gemm_any.cu", symbol=f"{symbol}_any",
             arguments=(arg("x", ptr, "input", index=0), *tensors, HALF_OUT, *PRODUCT_DIMS,
                        *((ACTIVATION,) if gated else ()), TRANS_B) + RESERVED,
-            grid=(ceil_div(out_dim(0), meta("BLOCK_M")), ceil_div(out_dim(1), meta("BLOCK_N"))), dtype="float16",
+            grid=(mul(ceil_div(out_dim(0), meta("BLOCK_M")), ceil_div(out_dim(1), meta("BLOCK_N"))),), dtype="float16",
             variants=(Variant("m64n64k32", num_warps=8, meta={"BLOCK_M": 64, "BLOCK_N": 64}),)))
         # CTA pairs: boxes are rows of 128 bytes; one variant for weights
         # given by output channel, one that turns a [K, N] constant at upload.

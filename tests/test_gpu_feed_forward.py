@@ -551,6 +551,22 @@ def test_offsets_past_32_bits(cuda):
         ff.assert_within(y[part].cpu().numpy(), ff.gated_result({**inputs, "x": inputs["x"][part]}, 0), "far rows")
 
 
+@pytest.mark.parametrize("op", ["GatedGemm", "QGemm", "QGatedGemm"])
+def test_more_columns_than_a_grid_dimension_of_tiles(cuda, op):
+    """The general form (odd K) over 65538 tiles of 64 columns, both ways round."""
+    import torch
+
+    wide = 65536 * 64 + 70
+    for m, n in ((2, wide), (wide, 2)):
+        rng = np.random.default_rng(21)
+        case, result = {"GatedGemm": (ff.gated_case, lambda i: ff.gated_result(i, ff.SILU)),
+                        "QGemm": (lambda *a: ff.qgemm_case(*a, True), ff.qgemm_result),
+                        "QGatedGemm": (ff.qgated_case, lambda i: ff.qgated_result(i, ff.SILU))}[op]
+        inputs = case(rng, m, 3, n)
+        (y,) = single_on_device(op, {name: torch.from_numpy(a).cuda() for name, a in inputs.items()}, transB=1)
+        ff.assert_within(y.cpu().numpy(), result(inputs), f"{m}x{n}")
+
+
 def single_on_device(op, tensors, **attributes):
     """One node over device tensors, without host copies of them."""
     import torch
