@@ -6,8 +6,8 @@
 // an integer. A row of zeros has s = 0 and q = 0. A row that holds an infinity
 // or a NaN has s = inf or NaN and q = 0, so that a product with it is NaN.
 //
-// One pass over HBM (3 bytes an element). A warp (two, four or eight for long
-// rows) takes whole rows and waits for no other one: each lane copies its
+// One pass over HBM (3 bytes an element). A warp (two to sixteen for long or
+// few rows) takes whole rows and waits for no other one: each lane copies its
 // vectors of 8 elements into a queue of its own in shared memory (cp.async),
 // 9 KB a warp, finds the row's maximum, and reads them back to write the
 // integers. So 216 KB of an SM's rows are under way while 24 warps compute,
@@ -174,6 +174,7 @@ __device__ __forceinline__ void quantize_rows(uint8_t* smem, const unsigned shor
   const int group_in_block = threadIdx.x >> kLanesLog2;
   const int lane = threadIdx.x & (kLanes - 1);
   constexpr int groups_a_block = kWarps >> kWarpsLog2;
+  if (kWarps % kGroupWarps != 0 && group_in_block >= groups_a_block) return;  // sixteen warps: eight are left over
   const long long groups = static_cast<long long>(gridDim.x) * groups_a_block;
   const long long group = static_cast<long long>(blockIdx.x) * groups_a_block + group_in_block;
   const long long total = static_cast<long long>(rows) * columns;
@@ -247,7 +248,7 @@ __device__ __forceinline__ void quantize_rows(uint8_t* smem, const unsigned shor
 }
 
 // One row by a block, element by element: tensors off 16 bytes (x) or 8 (q), and
-// rows longer than the queues of eight warps.
+// rows longer than the queues of sixteen warps.
 __device__ __forceinline__ void quantize_row_unaligned(const unsigned short* __restrict__ x,
                                                        signed char* __restrict__ q, float* __restrict__ scale,
                                                        long long row, int columns, uint32_t* shared) {
@@ -276,28 +277,25 @@ ctb_quantize_rows_f16(const unsigned short* x, signed char* q, float* scale, int
   uint32_t* shared = reinterpret_cast<uint32_t*>(smem + kWarps * kSlots * 512);
   // At most: a row of a length that 8 does not divide may begin inside a vector.
   const int vectors = columns % 8 == 0 ? columns / 8 : (columns + 14) / 8;
-  if (!ctb::aligned16(x) || (reinterpret_cast<uintptr_t>(q) & 7u) != 0 || vectors > 8 * 32 * kSlots) {
+  if (!ctb::aligned16(x) || (reinterpret_cast<uintptr_t>(q) & 7u) != 0 || vectors > 16 * 32 * kSlots) {
     for (int row = blockIdx.x; row < rows; row += gridDim.x) quantize_row_unaligned(x, q, scale, row, columns, shared);
     return;
   }
   // Warps a row: those that finish first, by rounds of rows over the groups of
   // warps and a row's slots plus two for its maximum, among those whose queues
-  // hold two rows (eight warps: one). 16384 rows of 2048: one warp 22 us, two
-  // 24; 2048 rows of 4096: four 9.1 us, two 10.5; 8 rows: eight.
-  int warps_log2 = 3, slots = (vectors + 255) >> 8, rounds = 1;
-  float least = INFINITY;
-#pragma unroll
-  for (int w = 3; w >= 0; --w) {
-    const int lane_vectors = (vectors + (32 << w) - 1) >> (5 + w);
-    const float turns = ceilf(__fdividef(static_cast<float>(rows), static_cast<float>(gridDim.x * (kWarps >> w))));
-    const float cost = turns * static_cast<float>(lane_vectors + 2);
-    if (cost < least && (w == 3 || lane_vectors <= kSlots / 2)) {
-      least = cost;
-      warps_log2 = w;
-      slots = lane_vectors;
-      rounds = static_cast<int>(turns);
-    }
-  }
+  // hold two rows (eight and sixteen warps: one). 16384 rows of 2048: one warp
+  // 22 us, two 24; 2048 rows of 4096: four 9.0 us, two 10.5; 8 rows of 12288:
+  // sixteen 2.9 us, eight 4.4 us; 2048 rows of 40000: sixteen 65 us, element by
+  // element 232 us.
+  // Lane w rates 2^w warps; ties go to the most.
+  const int w = min(static_cast<int>(threadIdx.x & 31), 4);
+  const int lane_vectors = (vectors + (32 << w) - 1) >> (5 + w);
+  const float turns = ceilf(__fdividef(static_cast<float>(rows), static_cast<float>(gridDim.x * (kWarps >> w))));
+  const unsigned cost = static_cast<unsigned>(fminf(turns * static_cast<float>(lane_vectors + 2), 4e8f));
+  const unsigned rated = lane_vectors <= (w >= 3 ? kSlots : kSlots / 2) ? cost * 8u + static_cast<unsigned>(4 - w) : ~0u;
+  const int warps_log2 = 4 - static_cast<int>(__reduce_min_sync(0xFFFFFFFFu, rated) & 7u);
+  const int slots = (vectors + (32 << warps_log2) - 1) >> (5 + warps_log2);
+  const int rounds = static_cast<int>(__shfl_sync(0xFFFFFFFFu, turns, warps_log2));
   if (warps_log2 == 0 && slots <= kSlots / 4) {
     quantize_rows<0, 4>(smem, x, q, scale, rows, columns, slots,
                          min(rounds, kSlots / 4 / slots), shared);
@@ -307,9 +305,13 @@ ctb_quantize_rows_f16(const unsigned short* x, signed char* q, float* scale, int
     quantize_rows<1, 2>(smem, x, q, scale, rows, columns, slots, 1, shared);
   } else if (warps_log2 == 2) {
     quantize_rows<2, 2>(smem, x, q, scale, rows, columns, slots, 1, shared);
-  } else if (slots <= kSlots / 2) {
+  } else if (warps_log2 == 3 && slots <= kSlots / 2) {
     quantize_rows<3, 2>(smem, x, q, scale, rows, columns, slots, 1, shared);
-  } else {
+  } else if (warps_log2 == 3) {
     quantize_rows<3, 1>(smem, x, q, scale, rows, columns, slots, 1, shared);
+  } else if (slots <= kSlots / 2) {
+    quantize_rows<4, 2>(smem, x, q, scale, rows, columns, slots, 1, shared);
+  } else {
+    quantize_rows<4, 1>(smem, x, q, scale, rows, columns, slots, 1, shared);
   }
 }

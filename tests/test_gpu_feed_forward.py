@@ -234,6 +234,16 @@ def check_quantize(x, **options):
     np.testing.assert_array_equal(got["q"], q)
 
 
+@pytest.mark.parametrize("shape", [(1, 36864), (3, 36871), (149, 12289), (2, 65529), (301, 40000), (2, 73728), (3, 73730)],
+                         ids=str)
+def test_quantize_long_rows(cuda, shape):
+    """Eight and sixteen warps a row, one or two rows in their queues, and rows
+    that no queue holds."""
+    x = np.random.default_rng(shape).standard_normal(shape).astype(np.float16)
+    x[-1, -1] = 30.0
+    check_quantize(x)
+
+
 def test_quantize_rows_ties_and_special_values(cuda):
     """Scales that are powers of two put quotients exactly on halves; FP16's
     smallest numbers; quotients next to a half; rows of infinity and NaN."""
