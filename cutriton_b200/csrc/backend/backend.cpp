@@ -110,11 +110,13 @@ bool ConstraintHolds(const KernelConstraint& c, const Node& node, const ValueLoo
       return v != nullptr && static_cast<int64_t>(v->tensor.shape.size()) == c.expected;
     }
     case KernelConstraintKind::kDimMultipleOf:
-    case KernelConstraintKind::kDimLessEqual: {
+    case KernelConstraintKind::kDimLessEqual:
+    case KernelConstraintKind::kDimGreaterEqual: {
       const ValueDesc* v = pick(c.tensor_is_output);
       if (v == nullptr || c.axis < 0 || static_cast<std::size_t>(c.axis) >= v->tensor.shape.size()) return false;
       const int64_t dim = v->tensor.shape[static_cast<std::size_t>(c.axis)];
-      return c.kind == KernelConstraintKind::kDimMultipleOf ? dim % c.expected == 0 : dim <= c.expected;
+      if (c.kind == KernelConstraintKind::kDimMultipleOf) return dim % c.expected == 0;
+      return c.kind == KernelConstraintKind::kDimLessEqual ? dim <= c.expected : dim >= c.expected;
     }
   }
   return false;

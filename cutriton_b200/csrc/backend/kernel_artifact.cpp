@@ -244,8 +244,9 @@ KernelConstraint ParseConstraint(const json::Value& v) {
     c.attribute_name = v.at("name").str();
     c.expected_list = IntList(v.at("value"));
     if (const auto* d = v.find("default")) c.default_list = IntList(*d);
-  } else if (kind == "dim_multiple_of" || kind == "dim_le") {
-    c.kind = kind == "dim_le" ? KernelConstraintKind::kDimLessEqual
+  } else if (kind == "dim_multiple_of" || kind == "dim_le" || kind == "dim_ge") {
+    c.kind = kind == "dim_ge"   ? KernelConstraintKind::kDimGreaterEqual
+             : kind == "dim_le" ? KernelConstraintKind::kDimLessEqual
                               : KernelConstraintKind::kDimMultipleOf;
     tensor_ref();
     c.axis = AsInt(v.at("axis"));

@@ -51,6 +51,7 @@ _CONSTRAINT_FIELDS = {
     "attribute_list_eq": {"kind", "name", "value", "default"},
     "dim_multiple_of": {"kind", "source", "index", "axis", "value", "at_run"},
     "dim_le": {"kind", "source", "index", "axis", "value", "at_run"},
+    "dim_ge": {"kind", "source", "index", "axis", "value", "at_run"},
     "input_is_constant": {"kind", "index"},
 }
 _GRID_FIELDS = {

@@ -613,11 +613,11 @@ def _product_specs() -> list[KernelSpec]:
                       Variant("m256k128b_turned", arg_overrides=turned,
                               constraints=(by_columns, *({"kind": "input_is_constant", "index": i} for i in weights)),
                               **pair))))
-        # Few rows, weights by output channel: chosen at run time, as M is what
-        # shape profiles leave open. Against the CTA pairs, 16 rows: gated
-        # 4096x12288 37.3 for 43.2 us, in 8 bits 21.5 for 23.8; 8-bit
-        # 12288x4096 12.9 for 14.9 and 1024x1024 3.3 for 3.9. A form of it for
-        # 32 rows took 44.9 for 42.7, 27.6 for 23.9 and 18.6 for 15.0.
+        # At most 16 rows: chosen at run time, as M is what shape profiles leave
+        # open. Against the CTA pairs, 16 rows: gated 4096x12288 37.3 for 43.2
+        # us, in 8 bits 21.5 for 23.8; 8-bit 12288x4096 12.9 for 14.9 and
+        # 1024x1024 3.3 for 3.9. A form of it for 32 rows took 44.9 for 42.7,
+        # 27.6 for 23.9 and 18.6 for 15.0.
         stream = dict(num_warps=16 if gated else 20, shared_memory_bytes=231424, programmatic_launch=True)
         few_rows = {"kind": "dim_le", "source": "input", "index": 0, "axis": 0, "value": 16, "at_run": 1}
         stream_turned = {a.name: {"prepack": "transpose_2d"} for a in matrices}
@@ -632,6 +632,36 @@ def _product_specs() -> list[KernelSpec]:
                       Variant("rows16_turned", arg_overrides=stream_turned,
                               constraints=(by_columns, *({"kind": "input_is_constant", "index": i} for i in weights)),
                               **stream))))
+        # 17 to 32 rows, of plain products whose K is split in four or eight 64:
+        # K over a cluster, split the most that leaves its CTAs resident at once
+        # (32 rows: 8-bit 12288x4096 in four 13.1, in two 17.4 us; gated
+        # 4096x12288 in two 35.9, in four 41.6). Eight parts pay up to 1536
+        # columns (gated 4096x1024 8.5 us for 10.9, 2048x2048 9.0 for 8.5).
+        # Against the CTA pairs, 32 rows: gated 4096x12288 35.9 for 42.3 us,
+        # 12288x1504 18.0 for 25.2, 2048x4096 10.5 for 10.8, 1024x4096 7.8 for
+        # 7.7; in 8 bits 22.8 for 23.9; 8-bit 12288x4096 12.7 for 15.0. With 64
+        # rows gated 4096x12288 took 42.7 for 43.3 us, in 8 bits 27.6 for 23.9;
+        # 8-bit 12288x4096 14.6 for 15.4, 4096x12288 15.9 for 14.9.
+        narrow_maps = [a for a in maps if a.name in ("tma_x64", "tma_x32", "tma_gate128", "tma_up128", "tma_w128")]
+        narrow_turned = {a.name: {"prepack": "transpose_2d"} for a in narrow_maps if not a.name.startswith("tma_x")}
+        for split, above, widest in ((8, 1, 1536), (4, 1537, 9472), (2, 9473, 18944), (1, 18945, 2**31 - 1)):
+            most = 64 if not gated and split >= 4 else 32
+            limits = ({"kind": "dim_ge", "source": "input", "index": 0, "axis": 0, "value": 17, "at_run": 1},
+                      {"kind": "dim_le", "source": "input", "index": 0, "axis": 0, "value": most, "at_run": 1},
+                      {"kind": "dim_ge", "source": "output", "index": 0, "axis": 1, "value": above},
+                      {"kind": "dim_le", "source": "output", "index": 0, "axis": 1, "value": widest})
+            narrow = dict(num_warps=6, shared_memory_bytes=110592 + 256 + 1024, programmatic_launch=True)
+            specs.append(KernelSpec(
+                kernel_id=f"{name}.{tag}.narrow{split}", op_type=op_type, version=1, source="product_narrow.cu",
+                symbol=f"{symbol}_narrow{split}",
+                arguments=(*narrow_maps, *vectors, HALF_OUT, *PRODUCT_DIMS, *((ACTIVATION,) if gated else ())) + RESERVED,
+                grid=(mul(literal(split), ceil_div(out_dim(1), literal(128))),), dtype="float16",
+                constraints=(rows_of_16_bytes, *limits),
+                variants=(Variant("rows64", constraints=(by_rows,), **narrow),
+                          Variant("rows64_turned", arg_overrides=narrow_turned,
+                                  constraints=(by_columns,
+                                               *({"kind": "input_is_constant", "index": i} for i in weights)),
+                                  **narrow))))
     # One block of 24 warps an SM: a queue of 9 KB a warp, and its maxima.
     specs.append(KernelSpec(
         kernel_id="quantize_rows.fp16", op_type="QuantizeRows", version=1, source="quantize.cu",

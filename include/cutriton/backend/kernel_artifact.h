@@ -8,7 +8,7 @@
 //   * argument source "tensor_map": the binder encodes a CUtensorMap for TMA;
 //   * argument field "prepack": the argument binds a host-side transformed copy
 //     of a constant input (e.g. weights pre-split into TF32 hi/lo halves);
-//   * constraints "attribute_list_eq", "dim_multiple_of", "dim_le",
+//   * constraints "attribute_list_eq", "dim_multiple_of", "dim_le", "dim_ge",
 //     "input_is_constant";
 //   * argument source "input_numel".
 
@@ -84,6 +84,7 @@ enum class KernelConstraintKind {
   kAttributeListEquals,
   kDimMultipleOf,
   kDimLessEqual,
+  kDimGreaterEqual,
   kInputIsConstant,
 };
 
@@ -99,7 +100,7 @@ struct KernelConstraint {
   int64_t default_value{0};
   std::vector<int64_t> expected_list;
   std::vector<int64_t> default_list;
-  // kDimMultipleOf / kDimLessEqual: holds or not at the shapes of a run, not
+  // The dimension kinds: holds or not at the shapes of a run, not
   // at those of the compilation (a dimension that shape profiles leave open).
   // Lowering admits the variant either way; the context chooses it when the
   // condition holds and never runs it when it does not.

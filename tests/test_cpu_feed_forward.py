@@ -217,6 +217,14 @@ def test_inner_sizes_off_16_bytes_take_the_general_form(k):
     assert len(op["candidates"]) == 1 and ".any:" in op["candidates"][0]
 
 
+@pytest.mark.parametrize("n,split", [(1, 8), (1536, 8), (1537, 4), (9472, 4), (9473, 2), (18944, 2), (18945, 1)])
+def test_one_split_of_k_for_each_width(n, split):
+    shapes = dict(x=("f2", (20, 32)), w_gate=("f2", (n, 32)), w_up=("f2", (n, 32)))
+    engine = ct.build_engine(ff.product_graph("GatedGemm", zeros(**shapes), transB=1))
+    narrow = [c for c in engine.op(0)["candidates"] if ".narrow" in c]
+    assert len(narrow) == 1 and f".narrow{split}:" in narrow[0]
+
+
 def test_at_run_constraint_is_part_of_the_pack_schema():
     from cutriton_b200 import kernel_sdk, kernel_specs
 
@@ -258,6 +266,12 @@ def test_launch_shapes_match_the_kernels():
                 assert f"constexpr int {name} = ({readers} + kJoinWarps) * 32;" in (folder / spec.source).read_text()
                 assert variant.num_warps == readers + constant(spec.source, "kJoinWarps")
                 assert variant.shared_memory_bytes == constant(spec.source, "kSharedBytes") <= 232448
+            elif spec.source == "product_narrow.cu":
+                assert variant.num_warps * 32 == constant(spec.source, "kThreads")
+                assert variant.shared_memory_bytes >= constant(spec.source, "kRingBytes") + 100 + 1023
+                assert 2 * (variant.shared_memory_bytes + 1024) <= 228 * 1024  # two blocks an SM
+                boxes = {a.name: a.source["box"][1] for a in spec.arguments if a.source["kind"] == "tensor_map"}
+                assert boxes.pop("tma_x64") == 64 and boxes.pop("tma_x32") == 32 and set(boxes.values()) == {128}
             elif spec.source == "quantize.cu":
                 warps = constant(spec.source, "kWarps")
                 assert variant.num_warps == warps

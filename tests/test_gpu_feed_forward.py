@@ -70,7 +70,7 @@ def check_product(op, inputs, result, constants=(), **attributes):
             y = runner.run(index)["y"]
         except ct.CutritonError as error:
             # A form for few rows, pinned where it does not apply.
-            assert error.code == ct.SHAPE_ERROR and "stream" in name, (name, error)
+            assert error.code == ct.SHAPE_ERROR and ("stream" in name or "narrow" in name), (name, error)
             continue
         if name.startswith("unfused"):
             continue  # rounds between its steps; see test_unfused_gated_gemm
@@ -105,6 +105,31 @@ def test_qgemm(cuda, size, bias):
 def test_qgated_gemm(cuda, size, activation):
     inputs = ff.qgated_case(np.random.default_rng(size), *size)
     check_product("QGatedGemm", inputs, ff.qgated_result(inputs, activation), activation=activation, transB=1)
+
+
+# 17 to 64 rows over every split of K: parts without a block of K, widths on both
+# sides of each limit and off a tile.
+NARROW = [(17, 16, 1), (32, 1040, 1536), (25, 16, 1537), (31, 4112, 2000), (32, 272, 9472), (18, 528, 9473),
+          (32, 144, 18945), (33, 2064, 1000), (64, 80, 1600), (63, 6160, 130)]
+
+
+@pytest.mark.parametrize("op", ["GatedGemm", "QGemm", "QGatedGemm"])
+@pytest.mark.parametrize("size", NARROW, ids=lambda s: "x".join(map(str, s)))
+def test_narrow_products(cuda, op, size):
+    m, k, n = size
+    case, result = {"GatedGemm": (ff.gated_case, lambda i: ff.gated_result(i, ff.GELU)),
+                    "QGemm": (lambda *a: ff.qgemm_case(*a, True), ff.qgemm_result),
+                    "QGatedGemm": (ff.qgated_case, lambda i: ff.qgated_result(i, ff.GELU))}[op]
+    inputs = case(np.random.default_rng(size), m, k, n)
+    attributes = {"transB": 1, **({} if op == "QGemm" else {"activation": ff.GELU})}
+    runner = Runner(ff.product_graph(op, inputs, **attributes), inputs)
+    runner.output("y", (m, n), np.float16)
+    y = runner.run()["y"]
+    name = runner.engine.op(0)["candidates"][runner.context.selected_candidate(0)]
+    split = 8 if n <= 1536 else 4 if n <= 9472 else 2 if n <= 18944 else 1
+    assert (f".narrow{split}:" in name) == (m <= 32 or (op == "QGemm" and split >= 4)), name
+    ff.assert_within(y, result(inputs), name)
+    np.testing.assert_array_equal(runner.run()["y"], y)
 
 
 @pytest.mark.parametrize("constant", [False, True])
@@ -152,7 +177,7 @@ def test_large_values_and_non_finite_rows(cuda):
                 try:
                     y = runner.run(index)["y"]
                 except ct.CutritonError as error:
-                    assert error.code == ct.SHAPE_ERROR and "stream" in name
+                    assert error.code == ct.SHAPE_ERROR and ("stream" in name or "narrow" in name)
                     continue
                 assert np.isnan(y[1]).all() and not np.isfinite(y[2]).any(), name
                 over = np.abs(expected) > 65600
@@ -192,7 +217,7 @@ def test_non_finite_weights_stay_in_their_column(cuda, activation, rows):
         try:
             y = runner.run(index)["y"]
         except ct.CutritonError as error:
-            assert error.code == ct.SHAPE_ERROR and "stream" in name
+            assert error.code == ct.SHAPE_ERROR and ("stream" in name or "narrow" in name)
             continue
         inside = good[np.abs(expected[:, good]).max(axis=0) < 65000]
         assert (np.abs(y[:, inside].astype(np.float64) - expected[:, inside]) <= tol[:, inside]).all(), name
