@@ -475,6 +475,42 @@ def test_replays_and_streams_give_the_same(cuda):
             assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("eight", [False, True])
+def test_narrow_products_between_other_kernels(cuda, eight):
+    """Blocks of 24 rows without profiling, so that their kernels start before
+    those in front end, on two streams at once: the results of single runs."""
+    import torch
+
+    from cutriton_b200 import workloads
+
+    build = workloads.build_gated_ffn_int8 if eight else workloads.build_gated_ffn
+    model = build(workloads.gated_ffn_weights(256, 2000, seed=9), 24)
+    engine = ct.build_engine(model, tuning_mode=ct.TUNING_DISABLED, enable_profiling=False)
+    contexts = [engine.create_context() for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    xs = [torch.from_numpy(workloads.ffn_input(24, 256, seed=s)).cuda() for s in range(2)]
+    ys = [torch.empty_like(x) for x in xs]
+    wants = []
+    for context, x, y in zip(contexts, xs, ys):
+        context.bind_tensor("x", x)
+        context.bind_tensor("output", y, output=True)
+        torch.cuda.synchronize()
+        context.run()
+        wants.append(y.clone())
+    names = [op["candidates"][contexts[0].selected_candidate(i)] for i, op in enumerate(engine.ops())]
+    assert any(".narrow4:" in name for name in names), names
+    for _ in range(20):
+        for y in ys:
+            y.zero_()
+        torch.cuda.synchronize()
+        for context, stream in zip(contexts, streams):
+            context.run_async(stream.cuda_stream)
+        for context in contexts:
+            context.synchronize()
+        for y, want in zip(ys, wants):
+            assert torch.equal(y, want)
+
+
 @pytest.mark.parametrize("rows", [4, 40])
 def test_tuner_chooses_among_the_forms_that_take_the_shape(cuda, tmp_path, rows):
     rng = np.random.default_rng(9)
