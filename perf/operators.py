@@ -184,18 +184,29 @@ def _compile(state):
 @functools.cache
 def _stream():
     """The stream of the program's steps (the legacy default stream cannot be
-    captured, so a program of this framework has one)."""
-    return torch.cuda.Stream()
+    captured, so a program of this framework has one), and the events that
+    order it with the caller's."""
+    return torch.cuda.Stream(), torch.cuda.Event(), torch.cuda.Event()
 
 
 # ---- one pass -----------------------------------------------------------------
 
 
 def run(state):
+    """Ordered with the current stream as torch's own operations are: the run
+    reads what that stream has written, and what follows on it reads the run's
+    outputs. An error that a kernel reports is raised by the context's next
+    synchronize, the one of the following run at the latest."""
     if own:
+        stream, before, after = _stream()
+        caller = torch.cuda.current_stream()
         # A context has one run in flight: its last one is taken in first.
         state["context"].synchronize()
-        state["context"].run_async(_stream().cuda_stream)
+        before.record(caller)
+        stream.wait_event(before)
+        state["context"].run_async(stream.cuda_stream)
+        after.record(stream)
+        caller.wait_event(after)
         return state["outputs"]
     case, t = state["case"], state["tensors"]
     if case["op"] == "gated":
