@@ -352,7 +352,8 @@ __device__ __forceinline__ void issue_mmas(uint8_t* smem, Barriers* bars, const 
   int s = 0;
   uint32_t phase = 0;
   bool ok = true;
-  for (int tile = pair, local = 0; tile < tiles && ok; tile += pairs, ++local) {
+  int local = 0;
+  for (int tile = pair; tile < tiles && ok; tile += pairs, ++local) {
     const int buf = local & 1;
     if (local >= 2 && !warp_wait(&bars->tmem_empty[buf], ((local >> 1) - 1) & 1, abort, scratch, 72)) {
       ok = false;
@@ -385,6 +386,11 @@ __device__ __forceinline__ void issue_mmas(uint8_t* smem, Barriers* bars, const 
     }
     if (ok && elect_one()) umma_commit_pair(smem_addr(&bars->tmem_full[buf]));
     __syncwarp();
+  }
+  // The peer's epilogue warps arrive here from afar: the last arrivals on both
+  // accumulators have landed before this CTA may leave.
+  for (int last = max(0, local - 2); ok && last < local; ++last) {
+    ok = warp_wait(&bars->tmem_empty[last & 1], (last >> 1) & 1, abort, scratch, 76);
   }
   if (!ok) {
     if (elect_one()) {
@@ -454,6 +460,15 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
           s = 0;
           phase ^= 1;
         }
+      }
+    }
+    // The leader's commits arrive on this CTA's stages: the last one on each has
+    // landed before the CTA may leave (a stage never used passes at once).
+    for (int i = 0; ok && i < sh.stages; ++i) {
+      ok = warp_wait(&bars->empty[s], phase, abort, op.scratch, 77);
+      if (++s == sh.stages) {
+        s = 0;
+        phase ^= 1;
       }
     }
     if (*abort && leader && lane == 0) {

@@ -663,3 +663,23 @@ def single_on_device(op, tensors, **attributes):
     torch.cuda.synchronize()
     context.run()
     return outputs
+
+
+@pytest.mark.parametrize("op", ["GatedGemm", "QGemm", "QGatedGemm"])
+def test_pairs_whose_second_half_has_no_rows(cuda, op):
+    """One or two blocks of K, one or two tiles a pair and rows for one CTA of it
+    only: its peer has arrived on all of its barriers before it leaves. Forty
+    runs one behind the other, all alike."""
+    case, result = {"GatedGemm": (ff.gated_case, lambda i: ff.gated_result(i, ff.SILU)),
+                    "QGemm": (lambda *a: ff.qgemm_case(*a, True), ff.qgemm_result),
+                    "QGatedGemm": (ff.qgated_case, lambda i: ff.qgated_result(i, ff.SILU))}[op]
+    for m, k, n in ((1, 16, 8), (33, 144, 40), (129, 16, 4800)):
+        inputs = case(np.random.default_rng((m, k, n)), m, k, n)
+        runner = Runner(ff.product_graph(op, inputs, transB=1), inputs, enable_profiling=False)
+        runner.output("y", (m, n), np.float16)
+        (pair,) = [i for i, c in enumerate(runner.engine.op(0)["candidates"]) if ".pair:" in c]
+        y = runner.run(pair)["y"]
+        ff.assert_within(y, result(inputs), f"{op} {m}x{k}x{n}")
+        for _ in range(40):
+            runner.context.run()
+        np.testing.assert_array_equal(runner.outputs["y"].cpu().numpy(), y)
