@@ -464,13 +464,8 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
     }
     // The leader's commits arrive on this CTA's stages: the last one on each has
     // landed before the CTA may leave (a stage never used passes at once).
-    for (int i = 0; ok && i < sh.stages; ++i) {
-      ok = warp_wait(&bars->empty[s], phase, abort, op.scratch, 77);
-      if (++s == sh.stages) {
-        s = 0;
-        phase ^= 1;
-      }
-    }
+    if (ok && lane < sh.stages) mbar_wait(&bars->empty[lane], lane < s ? phase ^ 1u : phase, abort, op.scratch, 77);
+    __syncwarp();
     if (*abort && leader && lane == 0) {
       // Let the issued copies land before shared memory is released (the
       // peer's too: the leader's barrier counts them). Bounded: a phase the
