@@ -31,20 +31,38 @@ __device__ __forceinline__ float exp_fast(float x) {
 // slower). silu_fast is -0 where exp(-g) overflows.
 __device__ __forceinline__ float silu_fast(float g) { return g * reciprocal(1.0f + exp_fast(-g)); }
 
-// erf-GELU by the formula of erf_as7126.
+// erf-GELU, g Phi(g) with Phi(g) = erfc(-g / sqrt 2) / 2. For g < 0 Phi is small
+// and is computed as such: 1 + erf would leave its rounding error, 2^-24, of
+// it (at -5, where Phi is 3e-7, a fifth). With t = 1 / (1 + 0.2975 |g|),
+//
+//   Phi(-|g|) exp(g^2 / 2) = P(t),
+//
+// P of degree 6 fitted here in the Chebyshev nodes of t for 0 <= |g| <= 13.3
+// by weighted least squares, the weights scaled by the errors until these are
+// even: 1.43e-6 relative. With the roundings of FP32, the reciprocal and the
+// exponent the result is right to 2^-18 + g^2 2^-23 of itself, down to -13.2,
+// where exp is below the normal range and the result is 0. As many
+// instructions as the sum with erf (8-bit 300x512x4096 8.60 us for 8.64, FP16
+// 333x1008x2731 11.12 for 11.02).
 __device__ __forceinline__ float gelu_fast(float g) {
-  const float z = fabsf(g) * 0.7071067811865476f;
-  const float t = reciprocal(fmaf(0.3275911f, z, 1.0f));
-  float poly = fmaf(1.061405429f, t, -1.453152027f);
-  poly = fmaf(poly, t, 1.421413741f);
-  poly = fmaf(poly, t, -0.284496736f);
-  poly = fmaf(poly, t, 0.254829592f);
-  const float erf = fmaf(-poly * t, exp_fast(-z * z), 1.0f);
-  return 0.5f * g * (1.0f + copysignf(erf, g));
+  const float t = reciprocal(fmaf(0.2975f, fabsf(g), 1.0f));
+  float poly = fmaf(-0.08747842209f, t, 0.2578530828f);
+  poly = fmaf(poly, t, -0.06899382892f);
+  poly = fmaf(poly, t, 0.1758866973f);
+  poly = fmaf(poly, t, 0.1019707022f);
+  poly = fmaf(poly, t, 0.1208796454f);
+  poly = fmaf(poly, t, -0.0001185836975f);
+  // exp(-g^2 / 2) = 2^(-g^2 log2(e) / 2)
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -0.7213475204f * g));
+  const float tail = poly * e;  // Phi(-|g|)
+  // Phi(g) is tail or 1 - tail; __fsub_rn is not contracted, so that every
+  // kernel rounds alike.
+  return g * fabsf(__fsub_rn(tail, g < 0.0f ? 0.0f : 1.0f));
 }
 
 __device__ __forceinline__ float gated(float gate, float up, int activation) {
-  return (activation == kSilu ? silu(gate) : gelu_erf(gate)) * up;
+  return (activation == kSilu ? silu(gate) : gelu_fast(gate)) * up;
 }
 
 // acc is the exact sum of 8-bit products; FP32 keeps 24 of its bits, more

@@ -141,3 +141,47 @@ def assert_within(actual: np.ndarray, result: tuple[np.ndarray, np.ndarray], wha
         i = np.unravel_index(np.argmax(np.where(bad, err / tol, 0)), err.shape)
         raise AssertionError(f"{what}: {int(bad.sum())} of {bad.size} outside tolerance; worst at {i}: {actual[i]} vs "
                              f"{expected[i]}, tolerance {tol[i]:.3e}")
+
+
+def gelu_tail_case(rng, op, m, n):
+    """Gates from -12 to -0.2 beside `up` projections that bring the products
+    back into FP16's normal range: one product a sum, so that gate and up
+    are exact in FP32 (in FP16 `up` ends at 65504, and so the gates at -5.8).
+    Returns inputs, and gate and up in 64 bits."""
+    k = 16
+    row = 1 + np.arange(m) % 3 / 64
+    if op == "GatedGemm":
+        g = -np.exp(rng.uniform(np.log(0.2), np.log(5.6), n)).astype(np.float16).astype(np.float64)
+        reach = np.abs(activate_tail(g))
+        u = np.minimum(1 / reach, 40000).astype(np.float16).astype(np.float64)
+        x, wg, wu = np.zeros((m, k), np.float16), np.zeros((n, k), np.float16), np.zeros((n, k), np.float16)
+        x[:, 3], wg[:, 3], wu[:, 3] = row, g, u
+        return {"x": x, "w_gate": wg, "w_up": wu}, np.outer(row, g), np.outer(row, u)
+    g = -np.exp(rng.uniform(np.log(0.2), np.log(12.0), n))
+    x, wg, wu = np.zeros((m, k), np.int8), np.zeros((n, k), np.int8), np.zeros((n, k), np.int8)
+    x[:, 5], wg[:, 5], wu[:, 5] = 127, -127, 127
+    x_scale = (row / 127).astype(np.float32)
+    gate_scale = (-g / 127).astype(np.float32)
+    up_scale = (1 / np.abs(activate_tail(g)) / 127).astype(np.float32)
+    gate = -127.0 * 127 * np.outer(x_scale.astype(np.float64), gate_scale.astype(np.float64))
+    up = 127.0 * 127 * np.outer(x_scale.astype(np.float64), up_scale.astype(np.float64))
+    return {"x": x, "x_scale": x_scale, "w_gate": wg, "gate_scale": gate_scale, "w_up": wu, "up_scale": up_scale}, gate, up
+
+
+def activate_tail(g: np.ndarray) -> np.ndarray:
+    """The erf-GELU in 64 bits without cancellation."""
+    import math
+
+    return g * 0.5 * np.vectorize(math.erfc)(-g / math.sqrt(2.0))
+
+
+def gelu_tail_result(gate, up):
+    """(result, tolerance), relative throughout. The activation in FP32: 2^-18 +
+    g^2 2^-23 (fit 1.43e-6, reciprocal, polynomial and exponential 2^-20 and
+    less together; the exponent's roundings grow with it). A gate off by d relative moves GELU by at most (g^2 + 2) d for
+    g < 0 (g phi / Phi < g^2 + 1 there): the scales' product and theirs, half a
+    step each, 2^-23 in all. The same 2^-23 on up, half a step for the final
+    product, and the rounding to FP16."""
+    y = activate_tail(gate) * up
+    unit = 2.0**-18 + gate**2 * 2.0**-23 + (gate**2 + 2) * 2.0**-23 + 2.0**-23 + 2.0**-24
+    return y, np.abs(y) * (unit + HALF) + HALF_MIN

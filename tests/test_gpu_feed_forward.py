@@ -683,3 +683,13 @@ def test_pairs_whose_second_half_has_no_rows(cuda, op):
         for _ in range(40):
             runner.context.run()
         np.testing.assert_array_equal(runner.outputs["y"].cpu().numpy(), y)
+
+
+@pytest.mark.parametrize("op", ["GatedGemm", "QGatedGemm"])
+@pytest.mark.parametrize("rows", [1, 12, 24, 150])
+def test_gelu_far_below_zero(cuda, op, rows):
+    """Every form (few rows, narrow, pairs, general) keeps the small values of
+    GELU to FP16's precision where a large up projection shows them."""
+    inputs, gate, up = ff.gelu_tail_case(np.random.default_rng(rows), op, rows, 700)
+    candidates = check_product(op, inputs, ff.gelu_tail_result(gate, up), activation=ff.GELU, transB=1)
+    assert any(".any:" in c for c in candidates)
