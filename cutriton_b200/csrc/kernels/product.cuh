@@ -8,28 +8,25 @@ namespace ctb {
 
 enum : int { kSilu = 0, kGelu = 1 };
 
-// g / (1 + exp(-g)); the denominator overflows to infinity below -88, where
-// the result is -0 to FP32's precision.
-__device__ __forceinline__ float silu(float g) { return g / (1.0f + __expf(-g)); }
-
 __device__ __forceinline__ float reciprocal(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
-// exp(x) as 2^(x log2 e), 2^-21 relative for the exponents that matter; results
-// below the normal range are 0.
+// exp(x) as 2^(x log2 e). The product's rounding and the constant's move the
+// exponent by up to |x| log2(e) 2^-23, so the result is right to |x| 2^-23 of
+// itself, and 2^-22 more for ex2.approx; results below the normal range are 0.
 __device__ __forceinline__ float exp_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
   return r;
 }
 
-// The activations of the tensor-core epilogues, in the fewest instructions
-// (one reciprocal for two gates took fewer special functions and was 2 %
-// slower). silu_fast is -0 where exp(-g) overflows.
-__device__ __forceinline__ float silu_fast(float g) { return g * reciprocal(1.0f + exp_fast(-g)); }
+// g / (1 + exp(-g)) in the fewest instructions (one reciprocal for two gates
+// took fewer special functions and was 2 % slower); -0 where exp(-g)
+// overflows or its reciprocal is below the normal range (g < -87).
+__device__ __forceinline__ float silu(float g) { return g * reciprocal(1.0f + exp_fast(-g)); }
 
 // erf-GELU, g Phi(g) with Phi(g) = erfc(-g / sqrt 2) / 2. For g < 0 Phi is small
 // and is computed as such: 1 + erf would leave its rounding error, 2^-24, of
@@ -44,7 +41,7 @@ __device__ __forceinline__ float silu_fast(float g) { return g * reciprocal(1.0f
 // where exp is below the normal range and the result is 0. As many
 // instructions as the sum with erf (8-bit 300x512x4096 8.60 us for 8.64, FP16
 // 333x1008x2731 11.12 for 11.02).
-__device__ __forceinline__ float gelu_fast(float g) {
+__device__ __forceinline__ float gelu(float g) {
   const float t = reciprocal(fmaf(0.2975f, fabsf(g), 1.0f));
   float poly = fmaf(-0.08747842209f, t, 0.2578530828f);
   poly = fmaf(poly, t, -0.06899382892f);
@@ -61,8 +58,10 @@ __device__ __forceinline__ float gelu_fast(float g) {
   return g * fabsf(__fsub_rn(tail, g < 0.0f ? 0.0f : 1.0f));
 }
 
+// Every form takes the activation from here, so that a token's result does not
+// depend on how many rows run beside it (but for the order of FP32 sums).
 __device__ __forceinline__ float gated(float gate, float up, int activation) {
-  return (activation == kSilu ? silu(gate) : gelu_fast(gate)) * up;
+  return (activation == kSilu ? silu(gate) : gelu(gate)) * up;
 }
 
 // acc is the exact sum of 8-bit products; FP32 keeps 24 of its bits, more

@@ -284,7 +284,7 @@ __device__ __forceinline__ void product_narrow(const Operands& op, const TmaDesc
         y = ctb::dequantized(total[e], row_scale, __ldg(op.w_scale[0] + column), bias);
         if (kGated) z = ctb::dequantized(up[e], row_scale, __ldg(op.w_scale[1] + column), 0.0f);
       }
-      if (kGated) y = (op.activation == ctb::kSilu ? ctb::silu_fast(y) : ctb::gelu_fast(y)) * z;
+      if (kGated) y = ctb::gated(y, z, op.activation);
       dst[column] = __float2half_rn(y);
     }
   }

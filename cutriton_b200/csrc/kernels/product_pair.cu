@@ -310,10 +310,10 @@ __device__ __forceinline__ void finish(const Operands& op, uint32_t (&v)[kChunk]
   if constexpr (kGated) {
     if (op.activation == ctb::kSilu) {
 #pragma unroll
-      for (int j = 0; j < kChunk; ++j) y[j] = ctb::silu_fast(y[j]) * __uint_as_float(u[j]);
+      for (int j = 0; j < kChunk; ++j) y[j] = ctb::silu(y[j]) * __uint_as_float(u[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < kChunk; ++j) y[j] = ctb::gelu_fast(y[j]) * __uint_as_float(u[j]);
+      for (int j = 0; j < kChunk; ++j) y[j] = ctb::gelu(y[j]) * __uint_as_float(u[j]);
     }
   }
 #pragma unroll
