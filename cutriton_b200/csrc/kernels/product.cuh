@@ -66,7 +66,9 @@ __device__ __forceinline__ float gated(float gate, float up, int activation) {
 
 // acc is the exact sum of 8-bit products; FP32 keeps 24 of its bits, more
 // than the FP16 result. The scales are multiplied first: their product is the
-// same for every kernel form, so all forms round alike.
+// same for every kernel form, so all forms round alike. They are read by plain
+// loads, not through the read-only path, whose memory has to be constant while
+// the grid runs: the kernel that writes them may still be running when it starts.
 __device__ __forceinline__ float dequantized(int acc, float row_scale, float column_scale, float bias) {
   return fmaf(static_cast<float>(acc), row_scale * column_scale, bias);
 }

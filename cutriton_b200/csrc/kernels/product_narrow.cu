@@ -272,7 +272,7 @@ __device__ __forceinline__ void product_narrow(const Operands& op, const TmaDesc
       add<T>(total, v[p]);
       if (kGated) add<T>(up, u[p]);
     }
-    const float row_scale = T::kBlock == 128 ? __ldg(op.x_scale + token) : 0.0f;
+    const float row_scale = T::kBlock == 128 ? op.x_scale[token] : 0.0f;
     __half* dst = op.out + static_cast<long long>(token) * op.n;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -281,8 +281,8 @@ __device__ __forceinline__ void product_narrow(const Operands& op, const TmaDesc
       float y = static_cast<float>(total[e]), z = static_cast<float>(up[e]);
       if constexpr (T::kBlock == 128) {
         const float bias = !kGated && op.bias != nullptr ? __half2float(op.bias[column]) : 0.0f;
-        y = ctb::dequantized(total[e], row_scale, __ldg(op.w_scale[0] + column), bias);
-        if (kGated) z = ctb::dequantized(up[e], row_scale, __ldg(op.w_scale[1] + column), 0.0f);
+        y = ctb::dequantized(total[e], row_scale, op.w_scale[0][column], bias);
+        if (kGated) z = ctb::dequantized(up[e], row_scale, op.w_scale[1][column], 0.0f);
       }
       if (kGated) y = ctb::gated(y, z, op.activation);
       dst[column] = __float2half_rn(y);

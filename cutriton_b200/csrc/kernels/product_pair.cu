@@ -290,8 +290,8 @@ __device__ __forceinline__ void finish(const Operands& op, uint32_t (&v)[kChunk]
   if constexpr (kInt8) {
     const int column = min(column0 + lane, op.n - 1);
     // A lane is a row: it gets the columns' scales from the lanes that loaded them.
-    const float c0 = __ldg(op.w_scale[0] + column);
-    const float c1 = kGated ? __ldg(op.w_scale[1] + column) : 0.0f;
+    const float c0 = op.w_scale[0][column];
+    const float c1 = kGated ? op.w_scale[1][column] : 0.0f;
     const float bias = !kGated && op.bias != nullptr ? __half2float(op.bias[column]) : 0.0f;
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) {
@@ -503,7 +503,7 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
       const int row0 = (2 * mt + static_cast<int>(rank)) * sh.rows + quarter * 32;
       const bool has_rows = quarter * 32 < sh.rows && row0 < op.m;
       const int n0 = nt * sh.columns;
-      const float row_scale = op.x_scale != nullptr && has_rows && row0 + lane < op.m ? __ldg(op.x_scale + row0 + lane) : 0.0f;
+      const float row_scale = op.x_scale != nullptr && has_rows && row0 + lane < op.m ? op.x_scale[row0 + lane] : 0.0f;
       const bool ready = mbar_wait(&bars->tmem_full[buf], (local >> 1) & 1, abort, op.scratch, 75);
       __syncwarp();
       if (!ready) break;

@@ -271,8 +271,8 @@ __device__ __forceinline__ void product_stream(uint8_t* smem, const Operands<T>&
     if (column >= op.n || column >= last * 8) continue;
     float scale = 0.0f, up_scale = 0.0f, bias = 0.0f;
     if (T::kPiece == 16) {
-      scale = __ldg(op.w_scale[0] + column);
-      if (kGated) up_scale = __ldg(op.w_scale[1] + column);
+      scale = op.w_scale[0][column];
+      if (kGated) up_scale = op.w_scale[1][column];
       if (!kGated && op.bias != nullptr) bias = __half2float(op.bias[column]);
     }
 #pragma unroll
@@ -281,7 +281,7 @@ __device__ __forceinline__ void product_stream(uint8_t* smem, const Operands<T>&
       if (token >= op.m) continue;
       float y = static_cast<float>(total[r]), u = static_cast<float>(up[r]);
       if constexpr (T::kPiece == 16) {
-        const float row_scale = __ldg(op.x_scale + token);
+        const float row_scale = op.x_scale[token];
         y = ctb::dequantized(total[r], row_scale, scale, bias);
         if (kGated) u = ctb::dequantized(up[r], row_scale, up_scale, 0.0f);
       }

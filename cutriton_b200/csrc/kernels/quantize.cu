@@ -167,8 +167,8 @@ __device__ __forceinline__ Row row_at(const unsigned short* x, signed char* q, l
 // queue, by groups of 2^kWarpsLog2 warps (with the number of warps known to the
 // compiler 16384x8192 takes 67 us instead of 75).
 template <int kWarpsLog2, int kAhead>
-__device__ __forceinline__ void quantize_rows(uint8_t* smem, const unsigned short* __restrict__ x,
-                                              signed char* __restrict__ q, float* __restrict__ scale, int rows,
+__device__ __forceinline__ void quantize_rows(uint8_t* smem, const unsigned short* x,
+                                              signed char* q, float* scale, int rows,
                                               int columns, int slots, int batch, uint32_t* shared) {
   constexpr int kGroupWarps = 1 << kWarpsLog2, kLanesLog2 = 5 + kWarpsLog2, kLanes = 1 << kLanesLog2;
   const int group_in_block = threadIdx.x >> kLanesLog2;
@@ -249,8 +249,7 @@ __device__ __forceinline__ void quantize_rows(uint8_t* smem, const unsigned shor
 
 // One row by a block, element by element: tensors off 16 bytes (x) or 8 (q), and
 // rows longer than the queues of sixteen warps.
-__device__ __forceinline__ void quantize_row_unaligned(const unsigned short* __restrict__ x,
-                                                       signed char* __restrict__ q, float* __restrict__ scale,
+__device__ __forceinline__ void quantize_row_unaligned(const unsigned short* x, signed char* q, float* scale,
                                                        long long row, int columns, uint32_t* shared) {
   const unsigned short* xr = x + row * columns;
   uint32_t m = 0;
@@ -260,9 +259,20 @@ __device__ __forceinline__ void quantize_row_unaligned(const unsigned short* __r
   if (threadIdx.x == 0) scale[row] = s;
   const bool regular = m != 0 && m < 0x7C00u;
   const float inv = regular ? __frcp_rn(s) : 0.0f;
-  for (int i = threadIdx.x; i < columns; i += kThreads) {
-    const float f = __half2float(__ushort_as_half(xr[i]));
-    q[row * columns + i] = regular ? static_cast<signed char>(settle(f, s, rintf(f * inv))) : 0;
+  // Four loads before four stores: x may not be read through the read-only path
+  // (its writer can still run when this grid starts), so the compiler keeps
+  // every load behind the stores in front of it.
+  const unsigned n = static_cast<unsigned>(columns);
+  for (unsigned i0 = threadIdx.x; i0 < n; i0 += 4 * kThreads) {
+    unsigned short v[4];
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j) v[j] = i0 + j * kThreads < n ? xr[i0 + j * kThreads] : 0;
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j) {
+      const unsigned i = i0 + j * kThreads;
+      const float f = __half2float(__ushort_as_half(v[j]));
+      if (i < n) q[row * columns + i] = regular ? static_cast<signed char>(settle(f, s, rintf(f * inv))) : 0;
+    }
   }
 }
 

@@ -361,3 +361,20 @@ def test_one_matrix_may_be_both_weights():
     model.add_node("node", "GatedGemm", ["x", "w", "w"], ["y"], transB=1)
     model.add_output("y")
     assert ct.build_engine(model).value_desc("y") == (ct.FLOAT16, (4, 24))
+
+
+def test_kernels_that_start_early_read_no_tensor_as_constant():
+    """Under programmatic launch a grid starts while the kernel in front of it
+    still writes, so its tensors are not constant while it runs: no
+    read-only-path loads in the sources of the forms that ask for it."""
+    from pathlib import Path
+
+    from cutriton_b200 import kernel_specs
+
+    folder = Path(kernel_specs.__file__).resolve().parent / "csrc" / "kernels"
+    ops = ("GatedGemm", "QGemm", "QGatedGemm", "QuantizeRows")
+    sources = {s.source for s in kernel_specs.all_specs() if s.op_type in ops and any(v.programmatic_launch for v in s.variants)}
+    assert sources == {"product_pair.cu", "product_stream.cu", "product_narrow.cu", "quantize.cu"}
+    for name in sources | {"product.cuh"}:
+        text = (folder / name).read_text()
+        assert "__ldg" not in text and "__restrict__" not in text and "ld.global.nc" not in text, name
