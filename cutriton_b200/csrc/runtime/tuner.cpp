@@ -254,17 +254,20 @@ Status TuneCandidates(const TuningTarget& target, const TuningConfig& config, st
   }
   for (std::size_t c : order) {
     if (kernels[c].empty() || !target.admitted[c]) continue;
-    for (int w = 0; w < std::max(1, config.warmup_iterations); ++w) CUTRITON_RETURN_IF_ERROR(launch(c));
+    Status ran = Status::OK();
+    for (int w = 0; ran.ok() && w < std::max(1, config.warmup_iterations); ++w) ran = launch(c);
     CUTRITON_RETURN_IF_ERROR(drv::Check(api.cuStreamSynchronize(timer.stream), "cuStreamSynchronize"));
-    // A candidate whose kernel reported an error (a shape or alignment
-    // outside its contract, an abandoned wait) is not eligible; the default
-    // candidate's error is the op's error.
+    // A candidate that the host could not bind or launch (an element count past
+    // 32 bits, a tensor map that does not fit) or whose kernel reported an error
+    // (a shape or alignment outside its contract, an abandoned wait) is not
+    // eligible; the default candidate's error is the op's error.
     if (target.take_device_error) {
       const Status device = target.take_device_error();
-      if (!device.ok()) {
-        if (c == fallback) return device;
-        continue;
-      }
+      if (ran.ok()) ran = device;
+    }
+    if (!ran.ok()) {
+      if (c == fallback) return ran;
+      continue;
     }
     std::vector<double> produced;
     CUTRITON_RETURN_IF_ERROR(ReadBack(output, &produced));

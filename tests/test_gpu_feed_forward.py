@@ -714,3 +714,38 @@ def test_a_token_does_not_depend_on_its_batch(cuda, activation):
                 continue
             whole = y if whole is None else whole
             assert np.array_equal(y, whole[:rows]), (rows, name, int((y != whole[:rows]).sum()))
+
+
+@pytest.mark.parametrize("rows", [4, 40])
+def test_tuner_skips_a_candidate_that_cannot_be_launched(cuda, tmp_path, rows):
+    """A pack whose general form binds a tensor map of the wrong rank: the host
+    refuses every launch of it, and tuning goes on among the others. Pinned, it
+    is the run's error."""
+    import json
+    import shutil
+    from pathlib import Path
+
+    pack = json.loads((Path(ct.PACK_DIR) / "pack.json").read_text())
+    pack["kernels"] = [k for k in pack["kernels"] if k["op_type"] == "QGemm"]
+    for kernel in pack["kernels"]:
+        target = tmp_path / "pack" / kernel["binary"]
+        target.parent.mkdir(parents=True, exist_ok=True)
+        shutil.copy(Path(ct.PACK_DIR) / kernel["binary"], target)
+        if kernel["kernel_id"] == "qgemm.i8.any":
+            kernel["arguments"][0] = {"name": "x", "type": "tensormap", "source": {
+                "kind": "tensor_map", "tensor": "input", "index": 0, "box": [32], "swizzle": 0}}
+    (tmp_path / "pack" / "pack.json").write_text(json.dumps(pack))
+    inputs = ff.qgemm_case(np.random.default_rng(14), rows, 256, 96, True)
+    runner = Runner(ff.product_graph("QGemm", inputs, transB=1), inputs, tuning_mode=ct.TUNING_TUNE_ON_MISS,
+                    tuning_cache_dir=str(tmp_path / "cache"), kernel_artifact_dir=str(tmp_path / "pack"))
+    runner.output("y", (rows, 96), np.float16)
+    ff.assert_within(runner.run()["y"], ff.qgemm_result(inputs), "tuned")
+    names = runner.engine.op(0)["candidates"]
+    (general,) = [i for i, name in enumerate(names) if ".any:" in name]
+    assert runner.context.selected_candidate(0) != general
+    (choice,) = (tmp_path / "cache").glob("*.json")
+    medians = json.loads(choice.read_text())["median_ms"]
+    assert medians[names[general]] is None and sum(m is not None for m in medians.values()) >= 2
+    with pytest.raises(ct.CutritonError) as error:
+        runner.run(general)
+    assert error.value.code == ct.SHAPE_ERROR
