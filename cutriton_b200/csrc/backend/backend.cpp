@@ -370,6 +370,10 @@ class CudaSm100Backend final : public Backend {
       steps.push_back({"Gemm", in, {projected}});
       steps.push_back({"Gelu", {projected}, {out}});
     } else if (op == "GatedGemm") {
+      // Gate, activation and up projection pass through FP16, which a node that
+      // was written as one op does not (a gate above 65504 is infinite here); one
+      // that the fusion made of these steps may run as them.
+      candidate->pinned_only = GetIntAttribute(node, "from_steps", 0) == 0;
       // The gate's slot serves the up projection once it is activated.
       const std::string gate = temp("gate", 0);
       const std::string activated = temp("activated", 1);

@@ -557,6 +557,7 @@ class GatedGemmFusionPass final : public GraphPass {
         mul.set_inputs(std::move(inputs));
         mul.SetAttribute("activation", activation);
         mul.SetAttribute("transB", tb);
+        mul.SetAttribute("from_steps", int64_t{1});
         return true;
       }
       return false;

@@ -490,6 +490,9 @@ Status ExecutionContext::PrepareTuning() {
     for (std::size_t i = 0; i < ops.size(); ++i) {
       const PlanOp& op = ops[i];
       if (op.candidates.size() < 2 || s.pins.count(i) != 0) continue;
+      for (std::size_t c = 0; c < op.candidates.size(); ++c) {
+        if (op.candidates[c].pinned_only) admitted[i][c] = 0;
+      }
       const Node& node = graph.nodes().at(static_cast<std::size_t>(op.node_id));
       const std::string key = runtime::TuningFingerprint(op, node, graph, device_id);
       std::optional<std::string> cached;

@@ -38,6 +38,9 @@ struct ExecutionCandidate {
   std::vector<PlanStep> steps;
   std::vector<CandidateTemporary> temporaries;
   bool is_default{false};
+  // Rounds between its steps where the op's definition does not: it runs when it
+  // is pinned, and the tuner leaves it out.
+  bool pinned_only{false};
 };
 
 }  // namespace cutriton

@@ -749,3 +749,36 @@ def test_tuner_skips_a_candidate_that_cannot_be_launched(cuda, tmp_path, rows):
     with pytest.raises(ct.CutritonError) as error:
         runner.run(general)
     assert error.value.code == ct.SHAPE_ERROR
+
+
+@pytest.mark.parametrize("from_steps", [False, True])
+def test_tuning_keeps_the_definition_of_a_gated_product(cuda, tmp_path, from_steps):
+    """K = 203 leaves the general form and the steps. A node written as one op
+    has one rounding, whatever is faster; the graph's own steps may run as such."""
+    import json
+
+    rng = np.random.default_rng(15)
+    inputs = ff.gated_case(rng, 200, 203, 256, trans_b=0)
+    weights = ("w_gate", "w_up")
+    model = ff.product_graph("GatedGemm", inputs, weights)
+    if from_steps:
+        model = ct.Model()
+        model.add_input("x", [200, 203], dtype=np.float16, layout="")
+        for name in weights:
+            model.add_constant(name, inputs[name], layout="")
+        model.add_node("gate", "Gemm", ["x", "w_gate"], ["g"])
+        model.add_node("act", "Silu", ["g"], ["a"])
+        model.add_node("up", "Gemm", ["x", "w_up"], ["u"])
+        model.add_node("product", "Mul", ["a", "u"], ["y"])
+        model.add_output("y")
+    runner = Runner(model, {"x": inputs["x"]}, tuning_mode=ct.TUNING_TUNE_ON_MISS, tuning_cache_dir=str(tmp_path))
+    runner.output("y", (200, 256), np.float16)
+    y = runner.run()["y"]
+    (op,) = runner.engine.ops()
+    assert op["op_type"] == "GatedGemm" and len(op["candidates"]) == 2
+    (choice,) = tmp_path.glob("*.json")
+    medians = json.loads(choice.read_text())["median_ms"]
+    assert (medians["unfused:gated_gemm"] is not None) == from_steps
+    if not from_steps:
+        ff.assert_within(y, ff.gated_result(inputs, ff.SILU, trans_b=0), "tuned")
+    runner.run(op["candidates"].index("unfused:gated_gemm"))
