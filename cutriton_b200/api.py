@@ -154,6 +154,8 @@ def _to_model(ir: dict[str, Any], shapes: dict[str, tuple[int, ...]], dtypes: di
                 raise UnsupportedModelError(f"{where}: only the exact (erf) GELU is supported")
             out = {}
         elif op in _PRODUCTS:
+            if float(attrs.get("alpha", 1.0)) != 1.0 or int(attrs.get("transA", 0)) != 0:
+                raise UnsupportedModelError(f"{where}: alpha != 1 and transA are not supported")
             out = {"transB": int(attrs.get("transB", 0))}
             if op != "QGemm":
                 activation = attrs.get("activation", "silu")

@@ -378,3 +378,26 @@ def test_kernels_that_start_early_read_no_tensor_as_constant():
     for name in sources | {"product.cuh"}:
         text = (folder / name).read_text()
         assert "__ldg" not in text and "__restrict__" not in text and "ld.global.nc" not in text, name
+
+
+@pytest.mark.parametrize("op", ["GatedGemm", "QGemm", "QGatedGemm"])
+@pytest.mark.parametrize("attribute", [{"transA": 1}, {"alpha": 0.5}], ids=str)
+def test_facade_refuses_a_turned_or_scaled_left_operand(tmp_path, op, attribute):
+    """Square operands, whose shapes fit either way round."""
+    import json
+
+    from cutriton_b200 import api
+
+    half = op == "GatedGemm"
+    names = {"GatedGemm": ["x", "a", "b"], "QGemm": ["x", "s", "a", "t"], "QGatedGemm": ["x", "s", "a", "t", "b", "t"]}[op]
+    dtypes = {n: "float32" if n in "st" else "float16" if half else "int8" for n in names}
+    graph = {"inputs": sorted(set(names)), "outputs": ["y"], "input_dtypes": dtypes,
+             "nodes": [{"name": "g", "op_type": op, "inputs": names, "outputs": ["y"]}]}
+    shapes = {n: (16,) if n in "st" else (16, 16) for n in names}
+    path = tmp_path / "g.json"
+    path.write_text(json.dumps(graph))
+    assert api.compile(path).native(shapes).value_desc("y") == (ct.FLOAT16, (16, 16))
+    graph["nodes"][0].update(attribute)
+    path.write_text(json.dumps(graph))
+    with pytest.raises(api.UnsupportedModelError):
+        api.compile(path).native(shapes)
