@@ -153,7 +153,7 @@ std::string VariantProblem(const KernelArtifact& artifact, const Node& node, con
     if (v == nullptr || !v->is_constant) return "prepacks argument '" + argument.name + "', which is not a constant";
   }
   for (std::size_t i = 0; i < artifact.constraints.size(); ++i) {
-    if (artifact.constraints[i].at_run) continue;  // the context's choice, at each run's shapes
+    if (!artifact.constraints[i].at_compilation) continue;  // the context's choice, at each run's shapes
     if (!ConstraintHolds(artifact.constraints[i], node, lookup)) return "constraint " + std::to_string(i) + " fails";
   }
   return "";
@@ -486,7 +486,7 @@ bool HoldsAtRun(const ExecutionCandidate& candidate, const Node& node, const Gra
     if (kernel == nullptr) continue;
     for (const KernelConstraint& c : kernel->artifact.constraints) {
       if (!c.at_run) continue;
-      if (any != nullptr) *any = true;
+      if (any != nullptr && !c.at_compilation) *any = true;
       holds = holds && ConstraintHolds(c, node, lookup);
     }
   }

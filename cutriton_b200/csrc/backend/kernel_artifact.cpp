@@ -252,7 +252,10 @@ KernelConstraint ParseConstraint(const json::Value& v) {
     c.axis = AsInt(v.at("axis"));
     c.expected = AsInt(v.at("value"));
     if (c.expected <= 0) throw std::runtime_error(kind + " value must be positive");
-    c.at_run = IntOr(v, "at_run", 0) != 0;
+    const int64_t at_run = IntOr(v, "at_run", 0);
+    if (at_run < 0 || at_run > 2) throw std::runtime_error(kind + " at_run must be 0, 1 or 2");
+    c.at_run = at_run != 0;
+    c.at_compilation = at_run != 1;
   } else if (kind == "input_is_constant") {
     c.kind = KernelConstraintKind::kInputIsConstant;
     c.tensor_index = AsInt(v.at("index"));

@@ -203,7 +203,8 @@ Status CheckBinding(const std::string& name, const TensorDesc& want, const Tenso
 
 // The candidate `op` runs at the shapes of `graph`: the pinned one; else the
 // first whose run-time constraints (it has some) hold; else the default of the
-// lowering. `admitted` tells for each candidate whether it takes the shapes.
+// lowering, or the first one that takes the shapes where that does not.
+// `admitted` tells for each candidate whether it takes the shapes.
 Status ChooseCandidate(const PlanOp& op, const Graph& graph, const std::size_t* pin, std::size_t* chosen,
                        std::vector<char>* admitted) {
   const Node& node = graph.nodes().at(static_cast<std::size_t>(op.node_id));
@@ -217,6 +218,10 @@ Status ChooseCandidate(const PlanOp& op, const Graph& graph, const std::size_t* 
       *chosen = c;
       found = true;
     }
+  }
+  if (!found && *chosen < op.candidates.size() && !(*admitted)[*chosen]) {
+    const auto first = std::find(admitted->begin(), admitted->end(), 1);
+    if (first != admitted->end()) *chosen = static_cast<std::size_t>(first - admitted->begin());
   }
   if (pin != nullptr) *chosen = *pin;
   if (*chosen < op.candidates.size() && !(*admitted)[*chosen]) {

@@ -597,7 +597,7 @@ def _product_specs() -> list[KernelSpec]:
         turned = {a.name: {"prepack": "transpose_2d"} for a in maps[3:-1]}
         columns = 32 if gated else 64  # of the narrowest tile
         rows_of_16_bytes = {"kind": "dim_multiple_of", "source": "input", "index": 0, "axis": 1,
-                            "value": 8 if tag == "fp16" else 16}
+                            "value": 8 if tag == "fp16" else 16, "at_run": 2}
         pair = dict(num_warps=18, shared_memory_bytes=196608 + 32768 + 256 + 1024, programmatic_launch=True)
         by_rows = {"kind": "attribute_i64_eq", "name": "transB", "value": 1, "default": 0}
         by_columns = {"kind": "attribute_i64_eq", "name": "transB", "value": 0, "default": 0}

@@ -90,7 +90,8 @@ std::shared_ptr<Backend> CreateCudaTritonBackend();
 Status RegisterBuiltinBackends();
 
 // Whether every at_run constraint of the candidate's kernels holds for `node`
-// at the shapes of `graph`; `any` (optional) tells whether it has some.
+// at the shapes of `graph`; `any` (optional) tells whether it has some that hold
+// or not at a run only.
 bool HoldsAtRun(const ExecutionCandidate& candidate, const Node& node, const Graph& graph, bool* any = nullptr);
 
 // True for target names served by the artifact-backed CUDA backend.

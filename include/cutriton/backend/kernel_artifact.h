@@ -100,10 +100,12 @@ struct KernelConstraint {
   int64_t default_value{0};
   std::vector<int64_t> expected_list;
   std::vector<int64_t> default_list;
-  // The dimension kinds: holds or not at the shapes of a run, not
-  // at those of the compilation (a dimension that shape profiles leave open).
-  // Lowering admits the variant either way; the context chooses it when the
-  // condition holds and never runs it when it does not.
+  // The dimension kinds, for dimensions that shape profiles leave open: where
+  // the condition has to hold. Pack field at_run: 0 at the compilation's shapes
+  // only; 1 at a run's shapes only (lowering admits the variant either way, the
+  // context chooses it when the condition holds); 2 at both. The context never
+  // runs a variant whose condition at a run does not hold.
+  bool at_compilation{true};
   bool at_run{false};
 };
 

@@ -782,3 +782,37 @@ def test_tuning_keeps_the_definition_of_a_gated_product(cuda, tmp_path, from_ste
     if not from_steps:
         ff.assert_within(y, ff.gated_result(inputs, ff.SILU, trans_b=0), "tuned")
     runner.run(op["candidates"].index("unfused:gated_gemm"))
+
+
+@pytest.mark.parametrize("rows", [4, 20, 70])
+def test_inner_sizes_of_one_profile_choose_their_form(cuda, rows):
+    """A profile that leaves K open: lengths that are no whole 16-byte rows take
+    the general form, the others the one of their row count."""
+    import torch
+
+    model = ct.Model()
+    shapes = {"x": (np.int8, lambda k: [rows, k]), "x_scale": (np.float32, lambda k: [rows]),
+              "w": (np.int8, lambda k: [24, k]), "w_scale": (np.float32, lambda k: [24])}
+    for name, (dtype, shape) in shapes.items():
+        model.add_input(name, shape(-1), dtype=dtype, layout="")
+    model.add_node("node", "QGemm", list(shapes), ["y"], transB=1)
+    model.add_output("y")
+    for name, (_, shape) in shapes.items():
+        model.add_shape_profile("inner", name, shape(16), shape(64), shape(300))
+    engine = ct.build_engine(model, tuning_mode=ct.TUNING_DISABLED)
+    context = engine.create_context()
+    for k in (64, 17, 300, 272, 18, 16):
+        inputs = ff.qgemm_case(np.random.default_rng(k), rows, k, 24, False)
+        for name, (_, shape) in shapes.items():
+            context.set_input_shape(name, shape(k))
+        context.resolve_shapes()
+        device = {name: torch.from_numpy(a).cuda() for name, a in inputs.items()}
+        y = torch.empty(rows, 24, dtype=torch.float16, device="cuda")
+        for name, tensor in device.items():
+            context.bind_tensor(name, tensor)
+        context.bind_tensor("y", y, output=True)
+        torch.cuda.synchronize()
+        context.run()
+        ff.assert_within(y.cpu().numpy(), ff.qgemm_result(inputs), f"{rows}x{k}")
+        chosen = engine.op(0)["candidates"][context.selected_candidate(0)]
+        assert (".any:" in chosen) == (k % 16 != 0), (k, chosen)
