@@ -69,7 +69,8 @@ struct __align__(8) Barriers {
 };
 
 struct Operands {
-  const TmaDescriptor* x;  // the box of 32 or 64 rows
+  const TmaDescriptor* x32;  // boxes of 32 and 64 rows
+  const TmaDescriptor* x64;  // (kMaxTokens = 64)
   const TmaDescriptor* w[2];
   const float* x_scale;
   const float* w_scale[2];
@@ -124,18 +125,19 @@ __device__ __forceinline__ void add(typename T::Sum (&sum)[4], uint4 v) {
   sum[3] += T::sum(v.w);
 }
 
-template <typename T, bool kGated, int kSplit>
-__device__ __forceinline__ void product_narrow(const Operands& op, const TmaDescriptor* x32, const TmaDescriptor* x64) {
+// kMaxTokens: rows of x that the form takes, 32 or 64.
+template <typename T, bool kGated, int kSplit, int kMaxTokens>
+__device__ __forceinline__ void product_narrow(const Operands& op) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
   Barriers* bars = reinterpret_cast<Barriers*>(smem + kRingBytes);
   volatile int* abort = &bars->abort;
-  constexpr int kMatrices = kGated ? 2 : 1, kMaxTokens = kGated ? 32 : 64;
+  constexpr int kMatrices = kGated ? 2 : 1;
   static_assert(kMatrices * kMaxTokens * kChannels * 4 <= kRingBytes, "the joined sums lie in the ring");
   constexpr uint32_t kTmemCols = kMatrices * kMaxTokens;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int tokens = kMaxTokens == 32 || op.m <= 32 ? 32 : 64;  // of the MMAs
-  const TmaDescriptor* x = kMaxTokens == 32 || op.m <= 32 ? x32 : x64;
+  const TmaDescriptor* x = tokens == 32 ? op.x32 : op.x64;
   const int x_bytes = tokens * kRowBytes;
   const int stage_bytes = x_bytes + kMatrices * kChannels * kRowBytes;  // a multiple of 1024
   constexpr int kWeightBytes = kMatrices * kChannels * kRowBytes;
@@ -158,7 +160,7 @@ __device__ __forceinline__ void product_narrow(const Operands& op, const TmaDesc
   }
   __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  // More rows are not this kernel's (the host offers it only up to 64).
+  // More rows are not this kernel's (the host does not offer it for them).
   const bool fits = op.m <= kMaxTokens;
 
   if (warp == 0 && fits) {
@@ -298,39 +300,40 @@ __device__ __forceinline__ void product_narrow(const Operands& op, const TmaDesc
 
 }  // namespace
 
-#define CTB_NARROW_KERNELS(split)                                                                                     \
-  extern "C" __global__ void __cluster_dims__(split, 1, 1) __launch_bounds__(kThreads, 2)                             \
-  ctb_gated_gemm_f16_narrow##split(const __grid_constant__ TmaDescriptor tma_x64,                                     \
-                                   const __grid_constant__ TmaDescriptor tma_x32,                                     \
-                                   const __grid_constant__ TmaDescriptor tma_gate,                                    \
-                                   const __grid_constant__ TmaDescriptor tma_up, __half* output, int m, int n, int k, \
-                                   int activation, CTB_RESERVED_PARAMS) {                                             \
-    (void)profile_scratch;                                                                                            \
-    const Operands op = {nullptr, {&tma_gate, &tma_up}, nullptr, {nullptr, nullptr}, nullptr, output, m, n, k,        \
-                         activation, runtime_scratch};                                                                \
-    product_narrow<Half, true, split>(op, &tma_x32, &tma_x64);                                                        \
-  }                                                                                                                   \
-  extern "C" __global__ void __cluster_dims__(split, 1, 1) __launch_bounds__(kThreads, 2)                             \
-  ctb_qgemm_i8_narrow##split(const __grid_constant__ TmaDescriptor tma_x64,                                           \
-                             const __grid_constant__ TmaDescriptor tma_x32,                                           \
-                             const __grid_constant__ TmaDescriptor tma_w, const float* x_scale, const float* w_scale, \
-                             const __half* bias, __half* output, int m, int n, int k, CTB_RESERVED_PARAMS) {          \
-    (void)profile_scratch;                                                                                            \
-    const Operands op = {nullptr, {&tma_w, nullptr}, x_scale, {w_scale, nullptr}, bias, output, m, n, k, 0,           \
-                         runtime_scratch};                                                                            \
-    product_narrow<Int8, false, split>(op, &tma_x32, &tma_x64);                                                       \
-  }                                                                                                                   \
-  extern "C" __global__ void __cluster_dims__(split, 1, 1) __launch_bounds__(kThreads, 2)                             \
-  ctb_qgated_gemm_i8_narrow##split(const __grid_constant__ TmaDescriptor tma_x64,                                     \
-                                   const __grid_constant__ TmaDescriptor tma_x32,                                     \
-                                   const __grid_constant__ TmaDescriptor tma_gate,                                    \
-                                   const __grid_constant__ TmaDescriptor tma_up, const float* x_scale,                \
-                                   const float* gate_scale, const float* up_scale, __half* output, int m, int n,      \
-                                   int k, int activation, CTB_RESERVED_PARAMS) {                                      \
-    (void)profile_scratch;                                                                                            \
-    const Operands op = {nullptr, {&tma_gate, &tma_up}, x_scale, {gate_scale, up_scale}, nullptr, output, m, n, k,    \
-                         activation, runtime_scratch};                                                                \
-    product_narrow<Int8, true, split>(op, &tma_x32, &tma_x64);                                                        \
+// One argument list for all splits: those of at most 32 rows take no x64.
+#define CTB_NARROW_KERNELS(split)                                                                                      \
+  extern "C" __global__ void __cluster_dims__(split, 1, 1) __launch_bounds__(kThreads, 2)                              \
+  ctb_gated_gemm_f16_narrow##split(const __grid_constant__ TmaDescriptor tma_x64,                                      \
+                                   const __grid_constant__ TmaDescriptor tma_x32,                                      \
+                                   const __grid_constant__ TmaDescriptor tma_gate,                                     \
+                                   const __grid_constant__ TmaDescriptor tma_up, __half* output, int m, int n, int k,  \
+                                   int activation, CTB_RESERVED_PARAMS) {                                              \
+    (void)profile_scratch;                                                                                             \
+    const Operands op = {&tma_x32, &tma_x64, {&tma_gate, &tma_up}, nullptr, {nullptr, nullptr}, nullptr, output,       \
+                         m, n, k, activation, runtime_scratch};                                                        \
+    product_narrow<Half, true, split, 32>(op);                                                                         \
+  }                                                                                                                    \
+  extern "C" __global__ void __cluster_dims__(split, 1, 1) __launch_bounds__(kThreads, 2)                              \
+  ctb_qgemm_i8_narrow##split(const __grid_constant__ TmaDescriptor tma_x64,                                            \
+                             const __grid_constant__ TmaDescriptor tma_x32,                                            \
+                             const __grid_constant__ TmaDescriptor tma_w, const float* x_scale, const float* w_scale,  \
+                             const __half* bias, __half* output, int m, int n, int k, CTB_RESERVED_PARAMS) {           \
+    (void)profile_scratch;                                                                                             \
+    const Operands op = {&tma_x32, &tma_x64, {&tma_w, nullptr}, x_scale, {w_scale, nullptr}, bias, output, m, n, k, 0, \
+                         runtime_scratch};                                                                             \
+    product_narrow<Int8, false, split, split >= 4 ? 64 : 32>(op);                                                      \
+  }                                                                                                                    \
+  extern "C" __global__ void __cluster_dims__(split, 1, 1) __launch_bounds__(kThreads, 2)                              \
+  ctb_qgated_gemm_i8_narrow##split(const __grid_constant__ TmaDescriptor tma_x64,                                      \
+                                   const __grid_constant__ TmaDescriptor tma_x32,                                      \
+                                   const __grid_constant__ TmaDescriptor tma_gate,                                     \
+                                   const __grid_constant__ TmaDescriptor tma_up, const float* x_scale,                 \
+                                   const float* gate_scale, const float* up_scale, __half* output, int m, int n,       \
+                                   int k, int activation, CTB_RESERVED_PARAMS) {                                       \
+    (void)profile_scratch;                                                                                             \
+    const Operands op = {&tma_x32, &tma_x64, {&tma_gate, &tma_up}, x_scale, {gate_scale, up_scale}, nullptr, output,   \
+                         m, n, k, activation, runtime_scratch};                                                        \
+    product_narrow<Int8, true, split, 32>(op);                                                                         \
   }
 
 CTB_NARROW_KERNELS(1)

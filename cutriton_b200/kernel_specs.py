@@ -644,7 +644,9 @@ def _product_specs() -> list[KernelSpec]:
         # 8-bit 12288x4096 14.6 for 15.4, 4096x12288 15.9 for 14.9.
         narrow_maps = [a for a in maps if a.name in ("tma_x64", "tma_x32", "tma_gate128", "tma_up128", "tma_w128")]
         narrow_turned = {a.name: {"prepack": "transpose_2d"} for a in narrow_maps if not a.name.startswith("tma_x")}
-        for split, above, widest in ((8, 1, 1536), (4, 1537, 9472), (2, 9473, 18944), (1, 18945, 2**31 - 1)):
+        resident = 2 * 148  # CTAs of this form at once: two an SM
+        widths = (1536, resident // 4 * 128, resident // 2 * 128, 2**31 - 1)
+        for split, above, widest in zip((8, 4, 2, 1), (1, *(w + 1 for w in widths)), widths):
             most = 64 if not gated and split >= 4 else 32
             limits = ({"kind": "dim_ge", "source": "input", "index": 0, "axis": 0, "value": 17, "at_run": 1},
                       {"kind": "dim_le", "source": "input", "index": 0, "axis": 0, "value": most, "at_run": 1},
@@ -657,8 +659,8 @@ def _product_specs() -> list[KernelSpec]:
                 arguments=(*narrow_maps, *vectors, HALF_OUT, *PRODUCT_DIMS, *((ACTIVATION,) if gated else ())) + RESERVED,
                 grid=(mul(literal(split), ceil_div(out_dim(1), literal(128))),), dtype="float16",
                 constraints=(rows_of_16_bytes, *limits),
-                variants=(Variant("rows64", constraints=(by_rows,), **narrow),
-                          Variant("rows64_turned", arg_overrides=narrow_turned,
+                variants=(Variant(f"rows{most}", constraints=(by_rows,), **narrow),
+                          Variant(f"rows{most}_turned", arg_overrides=narrow_turned,
                                   constraints=(by_columns,
                                                *({"kind": "input_is_constant", "index": i} for i in weights)),
                                   **narrow))))

@@ -401,3 +401,12 @@ def test_facade_refuses_a_turned_or_scaled_left_operand(tmp_path, op, attribute)
     path.write_text(json.dumps(graph))
     with pytest.raises(api.UnsupportedModelError):
         api.compile(path).native(shapes)
+
+
+def test_narrow_variants_are_named_by_the_rows_they_take():
+    from cutriton_b200 import kernel_specs
+
+    for spec in kernel_specs.all_specs():
+        if spec.source == "product_narrow.cu":
+            (most,) = [c["value"] for c in spec.constraints if c["kind"] == "dim_le" and c["source"] == "input"]
+            assert [v.variant_id for v in spec.variants] == [f"rows{most}", f"rows{most}_turned"], spec.kernel_id
