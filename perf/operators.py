@@ -202,8 +202,9 @@ def run(state):
         caller = torch.cuda.current_stream()
         # A context has one run in flight: its last one is taken in first.
         state["context"].synchronize()
-        before.record(caller)
-        stream.wait_event(before)
+        if not caller.query():  # (finished work needs no event)
+            before.record(caller)
+            stream.wait_event(before)
         state["context"].run_async(stream.cuda_stream)
         after.record(stream)
         caller.wait_event(after)
