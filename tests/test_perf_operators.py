@@ -17,10 +17,11 @@ def own(monkeypatch):
     operators._engine.cache_clear()
 
 
-def test_a_run_waits_for_the_caller_and_the_caller_for_it(own, monkeypatch):
+@pytest.mark.parametrize("idle", [False, True])
+def test_a_run_waits_for_the_caller_and_the_caller_for_it(own, monkeypatch, idle):
     """On recorded calls: the run's stream waits for the current one before the
-    run, the current one for the run's after it, and the context's last run is
-    taken in first."""
+    run (unless that has nothing left to do), the current one for the run's
+    after it, and the context's last run is taken in first."""
     import torch
 
     log = []
@@ -32,6 +33,9 @@ def test_a_run_waits_for_the_caller_and_the_caller_for_it(own, monkeypatch):
     class Stream:
         def __init__(self, name="side"):
             self.name, self.cuda_stream = name, name
+
+        def query(self):
+            return idle
 
         def wait_event(self, event):
             log.append((self.name, "waits for", event.of))
@@ -52,7 +56,7 @@ def test_a_run_waits_for_the_caller_and_the_caller_for_it(own, monkeypatch):
     outputs = [object()]
     assert operators.run({"context": Context(), "outputs": outputs}) is outputs
     assert log[0] == "synchronize"
-    assert log[1:] == [("side", "waits for", "caller"), ("run", "side"), ("caller", "waits for", "side")]
+    assert log[1:] == [("side", "waits for", "caller")][idle:] + [("run", "side"), ("caller", "waits for", "side")]
 
 
 @pytest.mark.gpu
