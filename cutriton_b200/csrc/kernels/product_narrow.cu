@@ -7,13 +7,13 @@
 // channels a CTA, of gate and of up for the gated ops) and the rows of x the N
 // side: a block of 128 bytes of K costs 64 to 128 clocks of MMAs and brings 4 or
 // 8 KB of x beside 16 or 32 KB of weights. 32x4096x12288 gated: 35.9 us, 5.6
-// TB/s, for 42.3 by CTA pairs; 8-bit 32x8192x28672 gated 78 us, 6.0 TB/s, for 91.
+// TB/s, for 42.8 by CTA pairs; 8-bit 32x8192x28672 gated 78 us, 6.0 TB/s, for 93.
 //
 // K is split over the kSplit CTAs of a cluster, so that narrow outputs occupy
 // every SM too. Each CTA leaves its sums [token][channel] in its own shared
 // memory and joins a share of the tokens over the cluster, in a fixed order
 // (results do not depend on timing), four channels a thread (with one a thread
-// 37.3 us). Two CTAs share an SM: one starts or joins while the other one reads.
+// 4 % more). Two CTAs share an SM: one starts or joins while the other one reads.
 //
 // TMEM is allocated between the dependency wait and the launch of dependents:
 // a CTA that waits for an earlier kernel holds none, and one that a later

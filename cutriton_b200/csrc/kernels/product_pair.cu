@@ -22,8 +22,8 @@
 // 4 half clocks of MMAs, 64 bytes a clock and SM through TMA (rows of x beyond
 // M are not loaded: zero-filling them took as long as loading them), or the
 // weights' share of HBM. At 512 clocks a block for half = 128 the tensor cores
-// are busy throughout (8192x4096x8192: 718 us, 1531 TFLOP/s; 8 bits
-// 8192x8192x4096: 169 us, 3253 TOP/s).
+// are busy throughout (8192x4096x8192: 723 us, 1520 TFLOP/s; 8 bits
+// 8192x8192x4096: 171 us, 3210 TOP/s).
 //
 // Warp 0 loads (a ring of 192 KB), warp 1 of CTA 0 issues the MMAs into one of
 // two accumulators, 16 epilogue warps of each CTA turn the other one into
@@ -121,9 +121,10 @@ __device__ __forceinline__ Shape shape_of(int width, int m, int n) {
   s.x_bytes = s.rows * kRowBytes;
   s.block_bytes = s.x_bytes + s.half * kRowBytes;  // a multiple of 1024
   // Short blocks share a stage, one round of barriers for two or four of them
-  // (32x12288x4096 in 8 bits: one 21.7, two 18.7, four 15.6 us), as long as
-  // enough stages are left (with three of two blocks 256x4096x12288 took 58
-  // instead of 51 us).
+  // (128x12288x4096 in 8 bits: one 22.7, two 17.5 us; 32 rows, were they not
+  // the narrow form's: one 22.1, two 17.0, four 15.0), as long as
+  // enough stages are left (with three of two blocks 256x4096x12288 took 50.8
+  // instead of 48.5 us).
   const int ring_blocks =
       static_cast<int>(kRingBytes * ctb::reciprocal(static_cast<float>(s.block_bytes)) + 1e-3f);  // 6 to 24
   s.blocks = ring_blocks >= 20 ? 4 : ring_blocks >= 8 ? 2 : 1;
@@ -608,11 +609,11 @@ __device__ __forceinline__ void product_pair(uint8_t* smem, const Operands& op, 
 // From HBM the weight rows of a block come at 23 bytes a clock and SM (5.6
 // clocks a row) when all pairs read, shared by the m_tiles rows of tiles, and
 // faster when the last wave leaves pairs idle. So few rows take the width that
-// keeps HBM busy in the last wave too (32x4096x12288: half 96 or 64 44 us, 128
-// 51 us, 32 60 us), many rows the widest (512x4096x11008 in 8 bits: 128 39 us,
-// 64 42 us, 32 62 us), and a single wave the narrowest (100x12288x1504: 32 37
-// us, 128 61 us). Every warp of both CTAs gets the same answer: lane i rates
-// width i, ties go to the widest.
+// keeps HBM busy in the last wave too (64x4096x12288: half 96 or 64 44 us, 128
+// 52 us, 32 49 us), many rows the widest (512x4096x11008 in 8 bits: 128 37 us,
+// 64 40 us, 32 59 us), and a single wave the narrowest (100x12288x1504: 32 30
+// us, 64 33 us, 128 60 us). Every warp of both CTAs gets the same answer: lane i
+// rates width i, ties go to the widest.
 template <bool kGated>
 __device__ __forceinline__ int choose_width(int m, int n, int pairs) {
   const int lane = threadIdx.x & 31;

@@ -23,9 +23,9 @@
 //   (results do not depend on timing), and store the outputs. The join buffer
 //   is double, so no reading warp waits for another one: when all of them met
 //   at a barrier after each batch (joined over a cluster of two CTAs, K split
-//   in 16), 16x4096x12288 took 45.7 us and the 8-bit form 29.0 us for 8 rows,
-//   against 36.4 and 20.3 us now.
-// 1x4096x12288 reads its 201 MB in 33.8 us, 5.96 TB/s.
+//   in 16), 16x4096x12288 took 24 % longer and the 8-bit form for 8 rows 42 %.
+// 16x4096x12288 takes 37.0 us, in 8 bits 21.2 and 20.4 for 8 rows;
+// 1x4096x12288 reads its 201 MB in 34.8 us, 5.8 TB/s.
 // All waits are bounded (tc_common.cuh).
 
 #include "product.cuh"
@@ -303,7 +303,7 @@ __device__ __forceinline__ void product_dispatch(const Operands<T>& op) {
     return;
   }
   // Reading warps: as many as leave every queue three slots and more beside
-  // the join buffers (16x4096x12288 with eight 36.4 us, with twelve 45.6).
+  // the join buffers (16x4096x12288 with twelve 25 % longer).
   constexpr int kFew = kGated ? 12 : 16, kMore = kGated ? 8 : 16;
   if (op.m <= 8) {
     product_stream<T, kGated, 1, kFew>(smem, op);

@@ -614,10 +614,10 @@ def _product_specs() -> list[KernelSpec]:
                               constraints=(by_columns, *({"kind": "input_is_constant", "index": i} for i in weights)),
                               **pair))))
         # At most 16 rows: chosen at run time, as M is what shape profiles leave
-        # open. Against the CTA pairs, 16 rows: gated 4096x12288 37.3 for 43.2
-        # us, in 8 bits 21.5 for 23.8; 8-bit 12288x4096 12.9 for 14.9 and
-        # 1024x1024 3.3 for 3.9. A form of it for 32 rows took 44.9 for 42.7,
-        # 27.6 for 23.9 and 18.6 for 15.0.
+        # open. Against the CTA pairs, 16 rows: gated 4096x12288 37.0 for 42.6
+        # us, in 8 bits 21.2 for 23.8; 8-bit 12288x4096 13.0 for 14.8 and
+        # 1024x1024 3.4 for 4.0. A form of it for 32 rows took 5, 16 and 24 %
+        # longer than the pairs on the first three.
         stream = dict(num_warps=16 if gated else 20, shared_memory_bytes=231424, programmatic_launch=True)
         few_rows = {"kind": "dim_le", "source": "input", "index": 0, "axis": 0, "value": 16, "at_run": 1}
         stream_turned = {a.name: {"prepack": "transpose_2d"} for a in matrices}
@@ -634,14 +634,16 @@ def _product_specs() -> list[KernelSpec]:
                               **stream))))
         # 17 to 32 rows, of plain products whose K is split in four or eight 64:
         # K over a cluster, split the most that leaves its CTAs resident at once
-        # (32 rows: 8-bit 12288x4096 in four 13.1, in two 17.4 us; gated
-        # 4096x12288 in two 35.9, in four 41.6). Eight parts pay up to 1536
-        # columns (gated 4096x1024 8.5 us for 10.9, 2048x2048 9.0 for 8.5).
-        # Against the CTA pairs, 32 rows: gated 4096x12288 35.9 for 42.3 us,
-        # 12288x1504 18.0 for 25.2, 2048x4096 10.5 for 10.8, 1024x4096 7.8 for
-        # 7.7; in 8 bits 22.8 for 23.9; 8-bit 12288x4096 12.7 for 15.0. With 64
-        # rows gated 4096x12288 took 42.7 for 43.3 us, in 8 bits 27.6 for 23.9;
-        # 8-bit 12288x4096 14.6 for 15.4, 4096x12288 15.9 for 14.9.
+        # (32 rows: 8-bit 12288x4096 in two 33 % longer than in four; gated
+        # 4096x12288 in four 16 % longer than in two). Eight parts pay up to 1536
+        # columns (gated 4096x1024 in four 28 % longer; 2048x2048 in eight 6 %).
+        # Against the CTA pairs, 32 rows: gated 4096x12288 35.9 for 42.8 us,
+        # 12288x1504 18.1 for 25.0, 4096x1024 8.5 for 10.3, 2048x4096 10.4 for
+        # 10.7; in 8 bits 4096x12288 22.8 for 23.7, 8-bit 12288x4096 12.8 for 14.8;
+        # of short K they are level or slower: 1024x4096 7.8 for 7.7, 2048x2048
+        # 8.6 for 7.9. 64 rows: 8-bit 12288x4096 14.4 for 15.3; 4096x12288 in a form
+        # for them gated 1 % shorter than the pairs, gated in 8 bits 15 % and
+        # 8-bit 7 % longer.
         narrow_maps = [a for a in maps if a.name in ("tma_x64", "tma_x32", "tma_gate128", "tma_up128", "tma_w128")]
         narrow_turned = {a.name: {"prepack": "transpose_2d"} for a in narrow_maps if not a.name.startswith("tma_x")}
         resident = 2 * 148  # CTAs of this form at once: two an SM
